@@ -83,19 +83,26 @@ __global__ void bn_stats_vec_kernel(const T *__restrict__ x,
 // LDS tree: a flat R-threads grid is only R/256 blocks (1-2 for BN-sized
 // R), which leaves one CU chewing through nb*R floats at latency — the
 // y-split is ~TY x more parallelism at identical determinism.  8
-// independent accumulators keep 8 loads in flight per thread.
+// independent accumulators keep 8 loads in flight per thread; the launch
+// bound leaves the registers for it (assuming 1024 threads a block, the
+// compiler waits for every load before it issues the next).
 template <int TX, int TY>
-__global__ void slab_reduce_kernel(const float *__restrict__ partial,
+__global__ void __launch_bounds__(TX * TY)
+slab_reduce_kernel(const float *__restrict__ partial,
                                    float *__restrict__ out, int nb, long R) {
     __shared__ float red[TY][TX];
     long r = (long)blockIdx.x * TX + threadIdx.x;
     float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < R) {
         int b = threadIdx.y;
-        for (; b + 7 * TY < nb; b += 8 * TY)
+        for (; b + 7 * TY < nb; b += 8 * TY) {
+            float pa[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                a[u] += partial[(long)(b + u * TY) * R + r];
+                pa[u] = partial[(long)(b + u * TY) * R + r];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a[u] += pa[u];
+        }
         for (; b < nb; b += TY) a[0] += partial[(long)b * R + r];
     }
     red[threadIdx.y][threadIdx.x] =
@@ -116,7 +123,8 @@ __global__ void slab_reduce_kernel(const float *__restrict__ partial,
 // carries the (sum, sumsq) PAIR for its channel so the ty==0 row can
 // finalize without a cross-column exchange.
 template <int TX, int TY>
-__global__ void bn_reduce_finalize_kernel(const float *__restrict__ partial,
+__global__ void __launch_bounds__(TX * TY)
+bn_reduce_finalize_kernel(const float *__restrict__ partial,
                                           int nb, int C, float n,
                                           float momentum, float eps,
                                           float *__restrict__ running_mean,
@@ -130,12 +138,19 @@ __global__ void bn_reduce_finalize_kernel(const float *__restrict__ partial,
     long R = 2L * C;
     if (c < C) {
         int b = threadIdx.y;
-        for (; b + 7 * TY < nb; b += 8 * TY)
+        for (; b + 7 * TY < nb; b += 8 * TY) {
+            float pa[8], pq[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                a[u] += partial[(long)(b + u * TY) * R + c];
-                q[u] += partial[(long)(b + u * TY) * R + C + c];
+                pa[u] = partial[(long)(b + u * TY) * R + c];
+                pq[u] = partial[(long)(b + u * TY) * R + C + c];
             }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                a[u] += pa[u];
+                q[u] += pq[u];
+            }
+        }
         for (; b < nb; b += TY) {
             a[0] += partial[(long)b * R + c];
             q[0] += partial[(long)b * R + C + c];
@@ -289,7 +304,8 @@ __global__ void bn_apply_kernel(const T *__restrict__ x,
 // ---- backward reduce: g = dy * relumask(y); out[0][c]=sum g,
 //      out[1][c]=sum g*xhat ----
 template <typename T, bool RELU, bool MASKED>
-__global__ void bn_bwd_reduce_vec_kernel(const T *__restrict__ dy,
+__global__ void __launch_bounds__(256)
+bn_bwd_reduce_vec_kernel(const T *__restrict__ dy,
                                          const T *__restrict__ y,
                                          const T *__restrict__ x,
                                          const unsigned char *__restrict__ mask,
@@ -335,6 +351,9 @@ __global__ void bn_bwd_reduce_vec_kernel(const T *__restrict__ dy,
                     vy1 = *reinterpret_cast<const s16x8 *>(y + i1);
                 }
             }
+            // all loads before the first use: left alone, the compiler puts
+            // one of them behind a wait for the others
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float g0 = s16_as_f32<T>(vdy0[e]), g1 = s16_as_f32<T>(vdy1[e]);
@@ -417,7 +436,8 @@ __global__ void bn_bwd_reduce_kernel(const T *__restrict__ dy,
 
 // ---- vectorized backward apply (C % 8 == 0) ----
 template <typename T, bool RELU, bool NEED_DRES, bool MASKED>
-__global__ void bn_bwd_apply_vec_kernel(const T *__restrict__ dy,
+__global__ void __launch_bounds__(256)
+bn_bwd_apply_vec_kernel(const T *__restrict__ dy,
                                         const T *__restrict__ y,
                                         const T *__restrict__ x,
                                         const unsigned char *__restrict__ mask,

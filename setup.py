@@ -59,7 +59,12 @@ setup(
             sources=SRC,
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+                # no packed float32 arithmetic: some forms of v_pk_*_f32 that
+                # the compiler makes from ordinary float code have given wrong
+                # results on this hardware
+                "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                         "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],
