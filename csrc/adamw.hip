@@ -1,0 +1,683 @@
+// sodkit — AdamW over many tensors at once, with the moments in 32 or in 8
+// bits.  One launch sweeps every parameter, whatever its type.
+//
+// The step, t counting the steps from one, every operation in float32 and
+// rounded by itself in this order (no contraction: the step gives the same
+// bits as the same operations one at a time, on any device, and so on every
+// rank):
+//
+//   g = float(grad) * (grad_scale * scale)
+//   m = b1*m + (1-b1)*g              v = b2*v + ((1-b2)*g)*g
+//   w = w*(1-lr*wd) - (lr/(1-b1^t)) * (m / (sqrt(v)*(1/sqrt(1-b2^t)) + eps))
+//
+// The scalars are computed in float64 and rounded once.  A parameter of 16
+// bits has a float32 master w and is its rounding; a float32 parameter is
+// its own w.
+//
+// It is bound by memory: 28 bytes an element, 16 with moments in 8 bits.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+#include "common.h"
+
+#pragma clang fp contract(off)
+
+namespace sodkit {
+namespace aw {
+
+constexpr int CHUNK = 4096;     // elements of a workgroup
+constexpr int BLOCK = 256;      // elements of an 8-bit block; tensors start at
+//                                 multiples of it in the states
+constexpr int ROWS = 160;       // table rows in one kernel's arguments
+
+// what stays of a tensor, and what may move from step to step
+struct Info {
+    long numel;
+    long state;                 // its first element in the moments
+    long master;                // and in the masters, -1: float32, its own
+    double wd;
+    long dtype;                 // 0 float32, 1 bfloat16, 2 float16
+};
+struct Row {
+    void *param;
+    const void *grad;           // null: no gradient, the tensor is left alone
+    long grad_dtype;
+    bool operator==(const Row &o) const {
+        return param == o.param && grad == o.grad && grad_dtype == o.grad_dtype;
+    }
+};
+struct Rows { Row row[ROWS]; };
+
+// Table rows travel as kernel arguments: no staging buffer to keep alive, and
+// a captured graph replays its own.
+__global__ void write_rows_kernel(const Rows rows, Row *__restrict__ out, int n) {
+    if ((int)threadIdx.x < n) out[threadIdx.x] = rows.row[threadIdx.x];
+}
+
+struct Args {
+    const Info *info;
+    const Row *rows;
+    const int2 *chunks;         // tensor, chunk of it
+    int *steps;                 // of every chunk: a workgroup counts its own,
+    //                             which spares a launch that counts for all
+    float *master;
+    const float *scale;         // null: 1; 0: skip
+    const float *lr_t;          // null: lr
+    double lr, b1, b2;
+    float fb1, fc1, fb2, fc2;   // b1, 1-b1, b2, 1-b2
+    float gscale, eps;
+    unsigned seed;
+};
+
+template <typename T> struct Vec4;  // 4 elements at any element's address
+template <> struct Vec4<float> {
+    typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct Vec4<__hip_bfloat16> {
+    typedef short type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct Vec4<__half> {
+    typedef short type __attribute__((ext_vector_type(4), aligned(2)));
+};
+
+template <typename T>
+SOD_DEVINL f32x4 load4(const T *p, long n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        auto v = *reinterpret_cast<const typename Vec4<T>::type *>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) r[e] = v[e];
+            else r[e] = s16_as_f32<T>(v[e]);
+        }
+    } else {
+        for (int e = 0; e < 3; ++e)
+            if (e < n) r[e] = ElemTraits<T>::to_f32(p[e]);
+    }
+    return r;
+}
+
+template <typename T>
+SOD_DEVINL void store4(T *p, long n, f32x4 r) {
+    if (n >= 4) {
+        typename Vec4<T>::type v;
+        if constexpr (sizeof(T) == 4) v = r;
+        else v = pack4<T>(r);
+        *reinterpret_cast<typename Vec4<T>::type *>(p) = v;
+    } else {
+        for (int e = 0; e < 3; ++e)
+            if (e < n) p[e] = ElemTraits<T>::from_f32(r[e]);
+    }
+}
+
+// b^t by squaring; b^t in float64 to a few units of its last place
+SOD_DEVINL double ipow(double b, unsigned t) {
+    double r = 1.0;
+    for (; t; t >>= 1) {
+        if (t & 1) r *= b;
+        b *= b;
+    }
+    return r;
+}
+
+// The scalars of a step, equal over a workgroup.
+struct Scalars { float rate, rbc2, keep; unsigned key; };
+
+// The finalizer of MurmurHash3 (Appleby, public domain).
+SOD_DEVINL unsigned mix32(unsigned h) {
+    h ^= h >> 16;
+    h *= 0x85EBCA6Bu;
+    h ^= h >> 13;
+    h *= 0xC2B2AE35u;
+    return h ^ (h >> 16);
+}
+
+SOD_DEVINL Scalars step_scalars(const Args &a, double wd, int tensor, long off) {
+    __shared__ Scalars sh;
+    if (threadIdx.x == 0) {
+        unsigned t = (unsigned)a.steps[blockIdx.x] + 1u;
+        a.steps[blockIdx.x] = (int)t;
+        double lr = a.lr_t ? (double)*a.lr_t : a.lr;
+        sh.rate = (float)(lr / (1.0 - ipow(a.b1, t)));
+        sh.rbc2 = (float)(1.0 / sqrt(1.0 - ipow(a.b2, t)));
+        sh.keep = (float)(1.0 - lr * wd);
+        unsigned k = mix32(a.seed + t * 0x9E3779B9u);
+        k = mix32(k + (unsigned)tensor);
+        sh.key = mix32(k + (unsigned)(off >> 32));
+    }
+    __syncthreads();
+    return sh;
+}
+
+SOD_DEVINL float moved(float w, float m, float r, float eps, const Scalars &s) {
+    float den = r * s.rbc2 + eps;
+    return w * s.keep - s.rate * (m / den);
+}
+
+// -------------------------------------------------------------- 32 bits
+
+template <typename P, typename G>
+SOD_DEVINL void chunk32(const Args &a, const Info &I, const Row &R, long off,
+                        float *m_, float *v_, float gs, const Scalars &s) {
+    P *p = reinterpret_cast<P *>(R.param);
+    const G *g_ = reinterpret_cast<const G *>(R.grad);
+    long end = min(off + (long)CHUNK, I.numel);
+    for (long i = off + threadIdx.x * 4; i < end; i += 1024) {
+        long n = I.numel - i;
+        f32x4 g = load4(g_ + i, n);
+        f32x4 m = *reinterpret_cast<f32x4 *>(m_ + I.state + i);
+        f32x4 v = *reinterpret_cast<f32x4 *>(v_ + I.state + i);
+        f32x4 w;
+        if constexpr (sizeof(P) == 4) w = load4(p + i, n);
+        else w = *reinterpret_cast<f32x4 *>(a.master + I.master + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x = g[e] * gs;
+            m[e] = a.fb1 * m[e] + a.fc1 * x;
+            v[e] = a.fb2 * v[e] + (a.fc2 * x) * x;
+            w[e] = moved(w[e], m[e], sqrtf(v[e]), a.eps, s);
+        }
+        // the states are padded past a tensor's end, its gradient reads 0 there
+        *reinterpret_cast<f32x4 *>(m_ + I.state + i) = m;
+        *reinterpret_cast<f32x4 *>(v_ + I.state + i) = v;
+        if constexpr (sizeof(P) != 4)
+            *reinterpret_cast<f32x4 *>(a.master + I.master + i) = w;
+        store4(p + i, n, w);
+    }
+}
+
+// call f with a tag of the parameter's and of the gradient's type
+struct F32 { using type = float; };
+struct BF16 { using type = __hip_bfloat16; };
+struct F16 { using type = __half; };
+template <typename P, typename F>
+SOD_DEVINL void by_grad(long g, F f) {
+    if (g == 0) f(P(), F32());
+    else if (g == 1) f(P(), BF16());
+    else f(P(), F16());
+}
+template <typename F>
+SOD_DEVINL void by_types(long p, long g, F f) {
+    if (p == 0) by_grad<F32>(g, f);
+    else if (p == 1) by_grad<BF16>(g, f);
+    else by_grad<F16>(g, f);
+}
+
+// false: nothing to do here
+SOD_DEVINL bool scaled(const Args &a, float &gs) {
+    gs = a.gscale;
+    if (a.scale != nullptr) {
+        // 0: the gradients overflowed.  Nothing moves, the step's count neither
+        float s = *a.scale;
+        if (s == 0.f) return false;
+        gs = gs * s;
+    }
+    return true;
+}
+
+__global__ void __launch_bounds__(256)
+adamw32_kernel(const Args a, float *__restrict__ m, float *__restrict__ v) {
+    float gs;
+    int2 c = a.chunks[blockIdx.x];
+    Info I = a.info[c.x];
+    Row R = a.rows[c.x];
+    if (R.grad == nullptr || !scaled(a, gs)) return;
+    long off = (long)c.y * CHUNK;
+    Scalars s = step_scalars(a, I.wd, c.x, off);
+    by_types(I.dtype, R.grad_dtype, [&](auto p, auto g) {
+        chunk32<typename decltype(p)::type, typename decltype(g)::type>(
+            a, I, R, off, m, v, gs, s);
+    });
+}
+
+// --------------------------------------------------------------- 8 bits
+//
+// A block of 256 elements, in the order of the tensor's storage, has two
+// float32 scales: its largest |m| and its largest r = sqrt(v).
+//   m  sign and 7 bits c: 0 is 0, else the float with the bits (c+889) << 20,
+//      8 steps an octave over 15.9 octaves, 127 standing for 1
+//   r  8 bits c: 0 is 0, else the float with the bits (c+1777) << 19, 16 steps
+//      an octave over 15.9 octaves, 255 standing for 1
+// times the scale.  Both are the top bits of a float32, so a code is a shift
+// away from its value and stochastic rounding is an addition of random bits
+// below the cut.
+//
+// Rounded to nearest, r would hardly ever move: with b2 = 0.999 a step changes
+// it by 0.05 %, and half a code step is 1.6 to 3.1 %.  The random bits are a
+// hash of seed, step, tensor and element.
+//
+// r is stored and not v: its codes then span 31.9 octaves of v, the next
+// step's sqrt(v) needs no second root, and it never rounds to zero unless it
+// is zero, which would leave m / eps.  A gradient that is not finite makes
+// its block's scales, and so its states, not finite.
+
+constexpr unsigned ONE = 0x3F800000u;
+
+template <int BIAS, int SHIFT>
+SOD_DEVINL float grid(unsigned c) {
+    return c ? __uint_as_float((c + BIAS) << SHIFT) : 0.f;
+}
+
+// x >= 0; at most the code of 1, below 1 for what is under the smallest code
+template <int BIAS, int SHIFT>
+SOD_DEVINL int code(float x, float inv, unsigned noise16) {
+    unsigned u = min(__float_as_uint(x * inv), ONE);
+    return (int)((u + (noise16 << (SHIFT - 16))) >> SHIFT) - BIAS;
+}
+
+// the largest bits over 32 lanes (floats >= 0 compare like their bits, and
+// NaN above all)
+SOD_DEVINL unsigned max32lanes(unsigned v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+        v = max(v, (unsigned)__shfl_xor((int)v, off, 64));
+    return v;
+}
+
+template <typename P, typename G>
+SOD_DEVINL void chunk8(const Args &a, const Info &I, const Row &R, long off,
+                       unsigned char *cm_, unsigned char *cr_, float2 *sc_,
+                       float gs, const Scalars &s) {
+    P *p = reinterpret_cast<P *>(R.param);
+    const G *g_ = reinterpret_cast<const G *>(R.grad);
+    long end = min(off + (long)CHUNK, I.numel);
+    // 32 lanes have a block; lanes past the end take part with zeros
+    for (long base = off; base < end; base += 2048) {
+        long i = base + threadIdx.x * 8;
+        long n = I.numel - i;
+        bool mine = (i & ~(long)(BLOCK - 1)) < I.numel;  // block has elements
+        f32x4 g[2], w[2];
+        uint2 cm = {0, 0}, cr = {0, 0};
+        float2 sc = make_float2(0.f, 0.f);
+        long blk = (I.state + i) / BLOCK;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            g[h] = load4(g_ + i + 4 * h, n - 4 * h);
+            if constexpr (sizeof(P) == 4) w[h] = load4(p + i + 4 * h, n - 4 * h);
+            else if (mine)
+                w[h] = *reinterpret_cast<f32x4 *>(a.master + I.master + i + 4 * h);
+            else w[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        if (mine) {
+            cm = *reinterpret_cast<uint2 *>(cm_ + I.state + i);
+            cr = *reinterpret_cast<uint2 *>(cr_ + I.state + i);
+            sc = sc_[blk];
+        }
+        float m[8], r[8];
+        unsigned mm = 0, mr = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            unsigned c = ((e < 4 ? cm.x : cm.y) >> (8 * (e & 3))) & 255u;
+            unsigned d = ((e < 4 ? cr.x : cr.y) >> (8 * (e & 3))) & 255u;
+            float m0 = grid<889, 20>(c & 127u) * sc.x;
+            if (c & 128u) m0 = -m0;
+            float r0 = grid<1777, 19>(d) * sc.y;
+            float x = g[e >> 2][e & 3] * gs;
+            m[e] = a.fb1 * m0 + a.fc1 * x;
+            float v = a.fb2 * (r0 * r0) + (a.fc2 * x) * x;
+            r[e] = sqrtf(v);
+            w[e >> 2][e & 3] = moved(w[e >> 2][e & 3], m[e], r[e], a.eps, s);
+            mm = max(mm, __float_as_uint(fabsf(m[e])));
+            mr = max(mr, __float_as_uint(fabsf(r[e])));
+        }
+        mm = max32lanes(mm);
+        mr = max32lanes(mr);
+        float sm = __uint_as_float(mm), sr = __uint_as_float(mr);
+        // NaN stays NaN: the comparison is false
+        float im = 1.f / (sm < 0x1p-100f ? 0x1p-100f : sm);
+        float ir = 1.f / (sr < 0x1p-100f ? 0x1p-100f : sr);
+        cm = {0, 0};
+        cr = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            unsigned h = mix32((unsigned)(i + e) + s.key);
+            int c = code<889, 20>(fabsf(m[e]), im, h >> 16);
+            if (c < 0) c = 0;
+            if (m[e] < 0.f && c > 0) c |= 128;
+            int d = code<1777, 19>(r[e], ir, h & 0xFFFFu);
+            if (d < 1) d = 1;
+            if (!(r[e] > 0.f)) d = 0;
+            (e < 4 ? cm.x : cm.y) |= (unsigned)c << (8 * (e & 3));
+            (e < 4 ? cr.x : cr.y) |= (unsigned)d << (8 * (e & 3));
+        }
+        if (mine) {
+            *reinterpret_cast<uint2 *>(cm_ + I.state + i) = cm;
+            *reinterpret_cast<uint2 *>(cr_ + I.state + i) = cr;
+            if ((threadIdx.x & 31) == 0) sc_[blk] = make_float2(sm, sr);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (sizeof(P) != 4)
+                if (mine)
+                    *reinterpret_cast<f32x4 *>(a.master + I.master + i + 4 * h) = w[h];
+            store4(p + i + 4 * h, n - 4 * h, w[h]);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256)
+adamw8_kernel(const Args a, unsigned char *__restrict__ cm,
+              unsigned char *__restrict__ cr, float2 *__restrict__ sc) {
+    float gs;
+    int2 c = a.chunks[blockIdx.x];
+    Info I = a.info[c.x];
+    Row R = a.rows[c.x];
+    if (R.grad == nullptr || !scaled(a, gs)) return;
+    long off = (long)c.y * CHUNK;
+    Scalars s = step_scalars(a, I.wd, c.x, off);
+    by_types(I.dtype, R.grad_dtype, [&](auto p, auto g) {
+        chunk8<typename decltype(p)::type, typename decltype(g)::type>(
+            a, I, R, off, cm, cr, sc, gs, s);
+    });
+}
+
+// the values that the codes stand for, rounded once to bfloat16
+__global__ void __launch_bounds__(256)
+adamw8_decode_kernel(const unsigned char *__restrict__ cm,
+                     const unsigned char *__restrict__ cr,
+                     const float2 *__restrict__ sc,
+                     __hip_bfloat16 *__restrict__ m,
+                     __hip_bfloat16 *__restrict__ v, long places) {
+    long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= places) return;
+    uint2 c2 = *reinterpret_cast<const uint2 *>(cm + i);
+    uint2 d2 = *reinterpret_cast<const uint2 *>(cr + i);
+    float2 s = sc[i / BLOCK];
+    f32x4 mo[2], vo[2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        unsigned c = ((e < 4 ? c2.x : c2.y) >> (8 * (e & 3))) & 255u;
+        unsigned d = ((e < 4 ? d2.x : d2.y) >> (8 * (e & 3))) & 255u;
+        float x = grid<889, 20>(c & 127u) * s.x;
+        float r = grid<1777, 19>(d) * s.y;
+        mo[e >> 2][e & 3] = c & 128u ? -x : x;
+        vo[e >> 2][e & 3] = r * r;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<s16x4 *>(m + i + 4 * h) = pack4<__hip_bfloat16>(mo[h]);
+        *reinterpret_cast<s16x4 *>(v + i + 4 * h) = pack4<__hip_bfloat16>(vo[h]);
+    }
+}
+
+// ---------------------------------------------------------------- plan
+
+int type_code(const torch::Tensor &t, const char *what) {
+    auto s = t.scalar_type();
+    TORCH_CHECK(s == torch::kFloat32 || s == torch::kBFloat16 ||
+                s == torch::kFloat16, "adamw: a ", what,
+                " must be float32, bfloat16 or float16, got ", s);
+    return s == torch::kFloat32 ? 0 : s == torch::kBFloat16 ? 1 : 2;
+}
+
+}  // namespace aw
+}  // namespace sodkit
+
+// The tables of one optimizer.  Addresses of parameters and gradients are
+// looked up on every step, on the host: a gradient that moved (autograd made
+// a new one) is seen, and its table written anew in front of the launch.
+class AdamWPlan {
+    using Row = sodkit::aw::Row;
+
+  public:
+    AdamWPlan(std::vector<torch::Tensor> params, std::vector<double> wd,
+              std::vector<int64_t> state, std::vector<int64_t> master,
+              torch::Tensor masters, std::vector<torch::Tensor> moments)
+        : params_(std::move(params)), masters_(masters),
+          moments_(std::move(moments)) {
+        using namespace sodkit::aw;
+        TORCH_CHECK(!params_.empty() && params_[0].is_cuda());
+        dev_ = params_[0].device();
+        c10::DeviceGuard guard(dev_);
+        size_t T = params_.size();
+        TORCH_CHECK(wd.size() == T && state.size() == T && master.size() == T);
+        std::vector<int64_t> info;          // Info's bytes
+        std::vector<int> chunks;
+        long places = 0, mplaces = 0;
+        for (size_t i = 0; i < T; ++i) {
+            auto &p = params_[i];
+            TORCH_CHECK(p.device() == dev_,
+                        "adamw: parameters must be on one device");
+            Info I;
+            I.numel = p.numel();
+            I.state = state[i];
+            I.master = master[i];
+            I.wd = wd[i];
+            I.dtype = type_code(p, "parameter");
+            dtypes_.push_back((int)I.dtype);
+            numels_.push_back(I.numel);
+            long pad = (I.numel + BLOCK - 1) / BLOCK * BLOCK;
+            TORCH_CHECK(I.state % BLOCK == 0 && I.state == places);
+            places += pad;
+            if (I.dtype != 0) {
+                TORCH_CHECK(I.master == mplaces);
+                mplaces += pad;
+            }
+            first_.push_back((int64_t)chunks.size() / 2);
+            for (long off = 0; off < I.numel; off += CHUNK) {
+                chunks.push_back((int)i);
+                chunks.push_back((int)(off / CHUNK));
+            }
+            int64_t raw[sizeof(Info) / 8];
+            memcpy(raw, &I, sizeof(I));
+            info.insert(info.end(), raw, raw + sizeof(Info) / 8);
+        }
+        n_chunks_ = (int64_t)chunks.size() / 2;
+        TORCH_CHECK(n_chunks_ < (1L << 31), "adamw: too many elements");
+        TORCH_CHECK(masters_.numel() == mplaces &&
+                    (moments_.size() == 2 || moments_.size() == 3));
+        for (int k = 0; k < 2; ++k)
+            TORCH_CHECK(moments_[k].numel() == places &&
+                        moments_[k].is_contiguous() &&
+                        moments_[k].device() == dev_);
+        if (moments_.size() == 3)
+            TORCH_CHECK(moments_[2].numel() == places / BLOCK * 2 &&
+                        moments_[2].is_contiguous());
+        auto i64 = torch::TensorOptions().dtype(torch::kInt64);
+        auto i32 = torch::TensorOptions().dtype(torch::kInt32);
+        info_ = torch::from_blob(info.data(), {(long)info.size()}, i64).to(dev_);
+        chunks_ = torch::from_blob(chunks.data(), {(long)chunks.size()}, i32)
+                      .to(dev_);
+        steps_ = torch::zeros({n_chunks_}, i32.device(dev_));
+        grads_.resize(T);
+    }
+
+    // where a gradient is read instead of the parameter's .grad (undefined
+    // or empty: there)
+    void set_grads(std::vector<torch::Tensor> grads) {
+        TORCH_CHECK(grads.size() == params_.size());
+        grads_ = std::move(grads);
+    }
+
+    // steps taken of every tensor; synchronizes
+    std::vector<int64_t> get_steps() const {
+        auto s = steps_.cpu();
+        std::vector<int64_t> out;
+        for (size_t i = 0; i < params_.size(); ++i)
+            out.push_back(numels_[i] ? s.data_ptr<int>()[first_[i]] : 0);
+        return out;
+    }
+
+    void set_steps(std::vector<int64_t> steps) {
+        TORCH_CHECK(steps.size() == params_.size());
+        auto s = torch::empty({n_chunks_}, torch::kInt32);
+        for (size_t i = 0; i < params_.size(); ++i) {
+            int64_t end = i + 1 < params_.size() ? first_[i + 1] : n_chunks_;
+            for (int64_t c = first_[i]; c < end; ++c)
+                s.data_ptr<int>()[c] = (int)steps[i];
+        }
+        steps_.copy_(s);
+    }
+
+    void step(double lr, torch::Tensor lr_t, double b1, double b2, double eps,
+              double gscale, torch::Tensor scale, int64_t seed) {
+        using namespace sodkit::aw;
+        if (n_chunks_ == 0) return;
+        c10::DeviceGuard guard(dev_);
+        auto stream = at::hip::getCurrentHIPStream();
+        Args a;
+        a.lr_t = scalar(lr_t, "lr");
+        a.scale = scalar(scale, "scale_t");
+        std::vector<torch::Tensor> copies;      // until the launch is queued
+        torch::Tensor rows = table(stream, copies);
+        a.info = reinterpret_cast<const Info *>(info_.data_ptr());
+        a.rows = reinterpret_cast<const Row *>(rows.data_ptr());
+        a.chunks = reinterpret_cast<const int2 *>(chunks_.data_ptr());
+        a.steps = steps_.data_ptr<int>();
+        a.master = masters_.numel() ? masters_.data_ptr<float>() : nullptr;
+        a.lr = lr;
+        a.b1 = b1;
+        a.b2 = b2;
+        a.fb1 = (float)b1;
+        a.fc1 = (float)(1.0 - b1);
+        a.fb2 = (float)b2;
+        a.fc2 = (float)(1.0 - b2);
+        a.eps = (float)eps;
+        a.gscale = (float)gscale;
+        a.seed = (unsigned)seed;
+        if (moments_.size() == 2)
+            hipLaunchKernelGGL(adamw32_kernel, dim3(n_chunks_), dim3(256), 0,
+                               stream.stream(), a, moments_[0].data_ptr<float>(),
+                               moments_[1].data_ptr<float>());
+        else
+            hipLaunchKernelGGL(adamw8_kernel, dim3(n_chunks_), dim3(256), 0,
+                               stream.stream(), a,
+                               moments_[0].data_ptr<unsigned char>(),
+                               moments_[1].data_ptr<unsigned char>(),
+                               reinterpret_cast<float2 *>(
+                                   moments_[2].data_ptr<float>()));
+    }
+
+  private:
+    const float *scalar(const torch::Tensor &t, const char *what) const {
+        if (!t.defined() || t.numel() == 0) return nullptr;
+        TORCH_CHECK(t.device() == dev_ && t.numel() == 1 &&
+                    t.scalar_type() == torch::kFloat32, "adamw: ", what,
+                    " must be a float32 scalar on the parameters' device");
+        return t.data_ptr<float>();
+    }
+
+    torch::Tensor table(const c10::hip::HIPStream &stream,
+                        std::vector<torch::Tensor> &copies) {
+        using namespace sodkit::aw;
+        size_t T = params_.size();
+        std::vector<Row> now(T);
+        for (size_t i = 0; i < T; ++i) {
+            auto &p = params_[i];
+            TORCH_CHECK(p.numel() == numels_[i] && p.device() == dev_ &&
+                        type_code(p, "parameter") == dtypes_[i] &&
+                        p.is_non_overlapping_and_dense(),
+                        "adamw: parameter ", i, " has changed its size, type, "
+                        "device or layout since the optimizer was made");
+            const auto &src = grads_[i];
+            torch::Tensor g = src.defined() && src.numel() ? src : p.grad();
+            now[i] = {p.data_ptr(), nullptr, 0};
+            if (!g.defined()) continue;
+            TORCH_CHECK(g.layout() == torch::kStrided && g.device() == dev_ &&
+                        g.sizes() == p.sizes(), "adamw: the gradient of "
+                        "parameter ", i, " must be dense, of its size and on "
+                        "its device");
+            now[i].grad_dtype = type_code(g, "gradient");
+            if (!same_order(g, p)) {
+                // elements are paired by their place in storage
+                g = torch::empty_strided(p.sizes(), p.strides(), g.options())
+                        .copy_(g);
+                copies.push_back(g);
+            }
+            now[i].grad = g.data_ptr();
+        }
+        if (rows_.defined() && now == host_) {
+            if (capturing()) kept_ = true;
+            else if (stream != made_on_)
+                rows_.record_stream(c10::Stream(c10::Stream::UNSAFE, dev_,
+                                                stream.id()));
+            return rows_;
+        }
+        // A table that a graph reads is never written again, and one that is
+        // made in a capture belongs to the graph alone.
+        auto rows = torch::empty(
+            {(long)(T * sizeof(Row))},
+            torch::TensorOptions().dtype(torch::kUInt8).device(dev_));
+        for (size_t at = 0; at < T; at += ROWS) {
+            Rows r;
+            int n = (int)std::min<size_t>(ROWS, T - at);
+            std::copy(now.begin() + at, now.begin() + at + n, r.row);
+            hipLaunchKernelGGL(write_rows_kernel, dim3(1), dim3(256), 0,
+                               stream.stream(), r,
+                               reinterpret_cast<Row *>(rows.data_ptr()) + at, n);
+        }
+        if (!capturing()) {
+            if (kept_) graphs_.push_back(rows_);
+            kept_ = false;
+            rows_ = rows;
+            host_ = now;
+            made_on_ = stream;
+        }
+        return rows;
+    }
+
+    // elements of equal place in storage are equal elements
+    static bool same_order(const torch::Tensor &a, const torch::Tensor &b) {
+        for (int64_t d = 0; d < a.dim(); ++d)
+            if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+        return true;
+    }
+
+    static bool capturing() {
+        hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+        auto st = at::hip::getCurrentHIPStream().stream();
+        return hipStreamIsCapturing(st, &s) == hipSuccess &&
+               s != hipStreamCaptureStatusNone;
+    }
+
+    c10::Device dev_ = c10::Device(c10::kCPU);
+    std::vector<torch::Tensor> params_, grads_;
+    torch::Tensor masters_;
+    std::vector<torch::Tensor> moments_;
+    std::vector<int> dtypes_;
+    std::vector<int64_t> numels_, first_;
+    int64_t n_chunks_ = 0;
+    torch::Tensor info_, chunks_, steps_, rows_;
+    std::vector<Row> host_;
+    bool kept_ = false;                     // a captured graph reads rows_
+    std::vector<torch::Tensor> graphs_;     // tables that graphs read
+    c10::hip::HIPStream made_on_ = at::hip::getDefaultHIPStream();
+};
+
+// {m, v} of moments in 8 bits, bfloat16, in the states' places
+std::vector<torch::Tensor> adamw8_decode(torch::Tensor cm, torch::Tensor cr,
+                                         torch::Tensor sc) {
+    using namespace sodkit::aw;
+    long n = cm.numel();
+    TORCH_CHECK(cm.is_cuda() && cr.numel() == n && n % BLOCK == 0 &&
+                sc.numel() == n / BLOCK * 2 && cm.is_contiguous() &&
+                cr.is_contiguous() && sc.is_contiguous());
+    c10::DeviceGuard guard(cm.device());
+    auto opt = cm.options().dtype(torch::kBFloat16);
+    auto m = torch::empty({n}, opt), v = torch::empty({n}, opt);
+    if (n == 0) return {m, v};
+    long g = (n / 8 + 255) / 256;
+    TORCH_CHECK(g < (1L << 31), "adamw: too many elements");
+    hipLaunchKernelGGL(adamw8_decode_kernel, dim3(g), dim3(256), 0,
+                       at::hip::getCurrentHIPStream().stream(),
+                       cm.data_ptr<unsigned char>(),
+                       cr.data_ptr<unsigned char>(),
+                       reinterpret_cast<const float2 *>(sc.data_ptr<float>()),
+                       reinterpret_cast<__hip_bfloat16 *>(m.data_ptr()),
+                       reinterpret_cast<__hip_bfloat16 *>(v.data_ptr()), n);
+    return {m, v};
+}
+
+void bind_adamw(pybind11::module_ &mod) {
+    pybind11::class_<AdamWPlan>(mod, "AdamWPlan")
+        .def(pybind11::init<std::vector<torch::Tensor>, std::vector<double>,
+                            std::vector<int64_t>, std::vector<int64_t>,
+                            torch::Tensor, std::vector<torch::Tensor>>())
+        .def("set_grads", &AdamWPlan::set_grads)
+        .def("get_steps", &AdamWPlan::get_steps)
+        .def("set_steps", &AdamWPlan::set_steps)
+        .def("step", &AdamWPlan::step);
+    mod.def("adamw8_decode", &adamw8_decode);
+}

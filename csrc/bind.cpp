@@ -119,6 +119,14 @@ void sgd_fused(torch::Tensor ptrs, torch::Tensor numels, torch::Tensor wds,
                double gscale, bool nesterov, torch::Tensor scale,
                torch::Tensor lr_t);
 
+std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads,
+                                     double prescale, double max_norm,
+                                     torch::Tensor loss_scale,
+                                     torch::Tensor good, torch::Tensor skips,
+                                     double growth);
+// AdamWPlan, adamw8_decode (csrc/adamw.hip)
+void bind_adamw(pybind11::module_ &mod);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "sodkit CDNA4 (gfx950/MI355X) kernels";
     m.def("conv2d_fwd", &conv2d_fwd);
@@ -156,6 +164,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("dynfilter_fwd", &dynfilter_fwd);
     m.def("dynfilter_bwd", &dynfilter_bwd);
     m.def("sgd_fused", &sgd_fused);
+    m.def("grad_norm", &grad_norm);
+    bind_adamw(m);
     m.def("multicopy_chunk_bytes", &multicopy_chunk_bytes);
     m.def("multicopy", &multicopy);
     m.def("multipermute", &multipermute);

@@ -1,0 +1,239 @@
+// sodkit — global gradient norm over many tensors at once, and from it the
+// multiplier of the optimizer's step: clipping, the dynamic loss scale, and
+// the skip of a step whose gradients overflowed.  No host round trip.
+//
+//   n    = prescale * sqrt(sum g^2) / L            L the loss scale, or 1
+//   mult = min(1, max_norm / (n + 1e-6)) / L       0 where n is not finite
+//
+// Squares are summed in 64 bits: a bfloat16 gradient of 2e19 has a square
+// past float32's range, which would read as an overflow that is none, and a
+// sum of 1e9 terms keeps its low digits.  Every block writes one partial sum
+// and a second kernel adds them in a fixed order (no atomics), so a repeated
+// call gives the same bits.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+#include "common.h"
+
+namespace sodkit {
+namespace gn {
+
+constexpr int SEGS = 160;       // tensors of one launch: 21 bytes each, and a
+//                                 kernel's arguments hold 4096
+constexpr int CHUNK = 8192;     // elements that a block reads at a time
+constexpr int MAX_BLOCKS = 2048;
+
+// The tensors travel as kernel arguments: nothing to allocate, to copy or to
+// keep, and a captured graph has its own.
+struct Segs {
+    const void *ptr[SEGS];
+    long numel[SEGS];
+    int first[SEGS];            // chunks of the tensors before
+    unsigned char dtype[SEGS];  // 0 float32, 1 bfloat16, 2 float16
+    int n, chunks;
+};
+
+template <typename T> struct Vec;   // 16 bytes, at any element's address
+template <> struct Vec<float> {
+    typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct Vec<__hip_bfloat16> {
+    typedef short type __attribute__((ext_vector_type(8), aligned(2)));
+};
+template <> struct Vec<__half> {
+    typedef short type __attribute__((ext_vector_type(8), aligned(2)));
+};
+
+SOD_DEVINL float elem(const Vec<float>::type &v, int i, float) { return v[i]; }
+template <typename T>
+SOD_DEVINL float elem(const typename Vec<T>::type &v, int i, T) {
+    return s16_as_f32<T>(v[i]);
+}
+
+template <typename T>
+SOD_DEVINL double chunk_sum(const T *p, long n) {
+    using V = typename Vec<T>::type;
+    constexpr int W = 16 / sizeof(T);
+    double a[4] = {0., 0., 0., 0.};
+    if (n == CHUNK) {
+#pragma unroll
+        for (int k = 0; k < CHUNK / W / 256; k += 4) {
+            V v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                v[u] = *reinterpret_cast<const V *>(
+                    p + ((k + u) * 256 + threadIdx.x) * W);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    double x = (double)elem(v[u], e, T());
+                    a[u] = fma(x, x, a[u]);
+                }
+        }
+    } else {
+        for (long i = threadIdx.x; i < n; i += 256) {
+            double x = (double)ElemTraits<T>::to_f32(p[i]);
+            a[0] = fma(x, x, a[0]);
+        }
+    }
+    return (a[0] + a[1]) + (a[2] + a[3]);
+}
+
+// sum over a block of 256; valid in thread 0
+SOD_DEVINL double block_sum(double s, double *red) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_down(s, off, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+__global__ void __launch_bounds__(256)
+norm_partial_kernel(const Segs segs, double *__restrict__ partial) {
+    __shared__ double red[4];
+    double s = 0.;
+    for (int c = blockIdx.x; c < segs.chunks; c += gridDim.x) {
+        int lo = 0, hi = segs.n - 1;        // the last tensor with first <= c
+        while (lo < hi) {
+            int mid = (lo + hi + 1) >> 1;
+            if (segs.first[mid] <= c) lo = mid; else hi = mid - 1;
+        }
+        long off = (long)(c - segs.first[lo]) * CHUNK;
+        long n = segs.numel[lo] - off;
+        if (n > CHUNK) n = CHUNK;
+        const void *p = segs.ptr[lo];
+        int d = segs.dtype[lo];
+        if (d == 0)
+            s += chunk_sum(reinterpret_cast<const float *>(p) + off, n);
+        else if (d == 1)
+            s += chunk_sum(reinterpret_cast<const __hip_bfloat16 *>(p) + off, n);
+        else
+            s += chunk_sum(reinterpret_cast<const __half *>(p) + off, n);
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+struct Final {
+    double prescale, max_norm;
+    float growth;               // good steps before the loss scale doubles
+    float *loss_scale, *good, *skips;   // null: 1 / not moved
+    float *norm, *mult;
+};
+
+SOD_DEVINL void finish(double sum, const Final &f) {
+    double L = f.loss_scale ? (double)*f.loss_scale : 1.0;
+    float norm = (float)(sqrt(sum) * f.prescale / L);
+    bool fine = isfinite(norm);
+    double m = 1.0;
+    if (f.max_norm > 0) m = fmin(f.max_norm / ((double)norm + 1e-6), 1.0);
+    // 0 means "skip the step": a finite norm never rounds to it
+    float mult = fmaxf((float)(m / L), 1.17549435e-38f);
+    *f.norm = norm;
+    *f.mult = fine ? mult : 0.f;
+    if (f.good) {
+        float good = fine ? *f.good + 1.f : 0.f;
+        bool grow = good >= f.growth;
+        float s = (float)L;
+        *f.loss_scale = !fine ? fmaxf(s * 0.5f, 1.f)
+                              : grow ? fminf(s * 2.f, 65536.f) : s;
+        *f.good = grow ? 0.f : good;
+        if (!fine) *f.skips += 1.f;
+    }
+}
+
+__global__ void __launch_bounds__(256)
+norm_final_kernel(const double *__restrict__ partial, int n, const Final f) {
+    __shared__ double red[4];
+    double s = 0.;
+    for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) finish(s, f);
+}
+
+float *scalar(const torch::Tensor &t, const char *what,
+              const c10::Device &dev) {
+    if (!t.defined() || t.numel() == 0) return nullptr;
+    TORCH_CHECK(t.device() == dev && t.scalar_type() == torch::kFloat32 &&
+                t.numel() == 1, "grad_norm: ", what,
+                " must be a float32 scalar on the gradients' device");
+    return t.data_ptr<float>();
+}
+
+}  // namespace gn
+}  // namespace sodkit
+
+// loss_scale / good / skips: float32 device scalars or empty; with good and
+// skips the three move as a dynamic loss scale does.  Returns {norm, mult}.
+std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads,
+                                     double prescale, double max_norm,
+                                     torch::Tensor loss_scale,
+                                     torch::Tensor good, torch::Tensor skips,
+                                     double growth) {
+    using namespace sodkit::gn;
+    TORCH_CHECK(!grads.empty(), "grad_norm: no gradients");
+    auto dev = grads[0].device();
+    TORCH_CHECK(dev.is_cuda(), "grad_norm: gradients must be on the GPU");
+    c10::DeviceGuard guard(dev);
+    std::vector<int> launches;             // the first tensor of each
+    std::vector<unsigned char> codes(grads.size());
+    for (size_t i = 0; i < grads.size(); ++i) {
+        auto &g = grads[i];
+        TORCH_CHECK(g.device() == dev && g.layout() == torch::kStrided,
+                    "grad_norm: gradients must be dense and on one device");
+        auto t = g.scalar_type();
+        TORCH_CHECK(t == torch::kFloat32 || t == torch::kBFloat16 ||
+                    t == torch::kFloat16, "grad_norm: gradients must be "
+                    "float32, bfloat16 or float16, got ", t);
+        codes[i] = t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : 2;
+        // the order of the elements is of no consequence, holes and overlaps are
+        if (!g.is_non_overlapping_and_dense()) g = g.contiguous();
+    }
+    auto opt = torch::TensorOptions().device(dev).dtype(torch::kFloat32);
+    auto norm = torch::empty({}, opt), mult = torch::empty({}, opt);
+    Final f;
+    f.prescale = prescale;
+    f.max_norm = max_norm;
+    f.growth = (float)growth;
+    f.loss_scale = scalar(loss_scale, "loss_scale", dev);
+    f.good = scalar(good, "good_steps", dev);
+    f.skips = scalar(skips, "skips", dev);
+    TORCH_CHECK(!f.good == !f.skips && (!f.good || f.loss_scale),
+                "grad_norm: good_steps and skips come together, and with a "
+                "loss_scale");
+    f.norm = norm.data_ptr<float>();
+    f.mult = mult.data_ptr<float>();
+
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    size_t n_launch = (grads.size() + SEGS - 1) / SEGS;
+    auto partial = torch::empty({(long)n_launch * MAX_BLOCKS},
+                                opt.dtype(torch::kFloat64));
+    double *out = partial.data_ptr<double>();
+    int blocks = 0;
+    for (size_t at = 0; at < grads.size(); at += SEGS) {
+        Segs s;
+        s.n = 0;
+        long chunks = 0;
+        for (size_t i = at; i < grads.size() && i < at + SEGS; ++i) {
+            if (grads[i].numel() == 0) continue;
+            s.ptr[s.n] = grads[i].data_ptr();
+            s.numel[s.n] = grads[i].numel();
+            s.first[s.n] = (int)chunks;
+            s.dtype[s.n++] = codes[i];
+            chunks += (grads[i].numel() + CHUNK - 1) / CHUNK;
+        }
+        TORCH_CHECK(chunks < (1L << 31), "grad_norm: too many elements");
+        if (chunks == 0) continue;
+        s.chunks = (int)chunks;
+        int g = (int)std::min<long>(chunks, MAX_BLOCKS);
+        hipLaunchKernelGGL(norm_partial_kernel, dim3(g), dim3(256), 0, stream,
+                           s, out + blocks);
+        blocks += g;
+    }
+    hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(256), 0, stream, out,
+                       blocks, f);
+    return {norm, mult};
+}

@@ -46,6 +46,8 @@ SRC = [
     "csrc/bilinear.hip",
     "csrc/loss.hip",
     "csrc/sgd.hip",
+    "csrc/adamw.hip",
+    "csrc/gradnorm.hip",
     "csrc/multicopy.hip",
     "csrc/maxpool.hip",
     "csrc/dynfilter.hip",

@@ -39,12 +39,18 @@ class Config:
     #                                      (deterministic DDP parity runs)
 
     # optimization
+    optimizer: str = "sgd"               # sgd | adamw (momentum / nesterov: sgd)
+    adam_beta1: float = 0.9
+    adam_beta2: float = 0.999
+    adam_eps: float = 1e-8
+    adam_state_bits: int = 32            # 32 | 8 (stochastically rounded codes)
     epoch_num: int = 3
     lr: float = 0.05
     momentum: float = 0.9
     weight_decay: float = 5e-4
     nesterov: bool = False
     sgd_trick: bool = True               # no weight-decay on bias/BN params
+    #                                      (either optimizer)
     lr_type: str = "poly"                # poly | const
     lr_power: float = 0.9
     warmup_iters: int = 0

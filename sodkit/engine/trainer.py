@@ -3,8 +3,8 @@ per-iter poly LR, (loss-scaled) fp16/bf16 step, custom gradient engine,
 checkpoint save/resume, distributed eval with MAE/F-measure.
 
 One step = load -> fwd -> hybrid loss -> bwd (buckets all-reduce on the side
-stream as they fill) -> fused SGD.  The 1/world average and any loss-scale
-unscale fold into the SGD grad_scale.
+stream as they fill) -> fused SGD or AdamW step (cfg.optimizer).  The 1/world
+average and any loss-scale unscale fold into the step's grad_scale.
 """
 
 from __future__ import annotations
@@ -81,10 +81,19 @@ class Solver:
             groups.append({"params": no_decay, "weight_decay": 0.0})
         else:
             groups[0]["params"] = decay + no_decay
-        self.optimizer = ops.SodSGD(groups, momentum=cfg.momentum,
-                                    weight_decay=cfg.weight_decay,
-                                    nesterov=cfg.nesterov)
-        # stable grad source for the fused-SGD pointer tables (deferred-grad
+        if cfg.optimizer == "adamw":
+            self.optimizer = ops.SodAdamW(
+                groups, betas=(cfg.adam_beta1, cfg.adam_beta2),
+                eps=cfg.adam_eps, weight_decay=cfg.weight_decay,
+                state_bits=cfg.adam_state_bits, seed=cfg.seed)
+        elif cfg.optimizer == "sgd":
+            self.optimizer = ops.SodSGD(groups, momentum=cfg.momentum,
+                                        weight_decay=cfg.weight_decay,
+                                        nesterov=cfg.nesterov)
+        else:
+            raise ValueError(f"unknown optimizer {cfg.optimizer!r}; "
+                             f"have 'sgd', 'adamw'")
+        # stable grad source for the fused step's pointer tables (deferred-grad
         # mode re-lands autograd's per-step grad tensors in these views)
         self.optimizer.grad_src = self.reducer.grad_views
 
@@ -161,11 +170,23 @@ class Solver:
         (0.0 => the kernel skips the update).  No ``.item()`` — the fp16
         [BJ:11] config runs sync-free (VERDICT r1 weak #4)."""
         cfg = self.cfg
+        accum = max(1, cfg.accum_steps)
+        if cfg.optimizer == "adamw":
+            # the same in two launches, none of which a captured graph replays
+            # through a memory clear (runs with sgd keep their arithmetic)
+            dyn = self.dynamic_scale
+            _, mult = ops.grad_norm(
+                [b.flat for b in self.reducer.buckets],
+                prescale=self.reducer.grad_scale / accum,
+                max_norm=cfg.grad_clip, loss_scale=self._scale_t,
+                good_steps=self._good_t if dyn else None,
+                skips=self._skips_t if dyn else None,
+                growth_interval=self._growth_interval)
+            return mult
         sq = None
         for b in self.reducer.buckets:
             n = b.flat.float().square().sum()
             sq = n if sq is None else sq + n
-        accum = max(1, cfg.accum_steps)
         # true (averaged, unscaled) grad norm; _scale_t is 1.0 unless fp16
         norm = torch.sqrt(sq) * (self.reducer.grad_scale / accum) / self._scale_t
         finite = torch.isfinite(norm)

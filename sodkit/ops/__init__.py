@@ -10,4 +10,6 @@ from .loss import hybrid_loss  # noqa: F401
 from .pool import maxpool2d_3x3s2  # noqa: F401
 from .dynfilter import dynamic_filter  # noqa: F401
 from .sgd import SodSGD, split_decay_groups  # noqa: F401
+from .adamw import SodAdamW  # noqa: F401
+from .gradnorm import grad_norm  # noqa: F401
 from . import reference  # noqa: F401

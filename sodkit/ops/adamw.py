@@ -1,0 +1,325 @@
+"""SodAdamW — AdamW over many tensors at once, with the moments in 32 or in 8
+bits: one launch over every parameter of every type (csrc/adamw.hip).  The
+same contract as SodSGD: fp32 masters of 16-bit parameters, the gradient
+average and the loss-scale unscale folded in as ``grad_scale``, a device
+multiplier that skips the step at 0, a device learning rate for captured steps.
+
+The step, t counting a parameter's steps from one, in float32 with every
+operation rounded by itself:
+
+    g = float(grad) * (grad_scale * scale_t)
+    m = b1*m + (1-b1)*g              v = b2*v + ((1-b2)*g)*g
+    w = w*(1-lr*wd) - (lr/(1-b1^t)) * (m / (sqrt(v)*(1/sqrt(1-b2^t)) + eps))
+
+Moments in 8 bits cost 2.03 bytes an element in place of 8.  A tensor is cut
+into blocks of 256 elements in the order of its storage, each with two float32
+scales, its largest |m| and its largest r = sqrt(v); m is a sign and 7 bits, 8
+steps an octave, r 8 bits, 16 steps an octave, both over 15.9 octaves below
+the scale.  Codes are rounded stochastically, by a hash of ``seed``, step,
+tensor and element: a run repeats itself, and all ranks agree.
+
+CPU path: ops.reference.adamw_step / adamw8_step, the same operations.
+"""
+
+from __future__ import annotations
+
+from typing import Iterable
+
+import torch
+
+from . import reference
+from ._backend import ext
+
+_BLOCK = 256  # elements of an 8-bit block (must match csrc/adamw.hip)
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _padded(n: int) -> int:
+    return -(-n // _BLOCK) * _BLOCK
+
+
+def _in_storage(t: torch.Tensor) -> torch.Tensor:
+    """The elements of a dense tensor in the order of its storage."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element of one stretch of storage, each once."""
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape)
+                               if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class SodAdamW:
+    """``param_groups``: dicts ``{"params": [...], "weight_decay": float}``, the
+    decay defaulting to ``weight_decay``.  ``state_bits``: 32 or 8.
+
+    The states lie in flat tensors, every parameter's at a multiple of 256
+    elements (the gaps are zero), in the groups' order: ``master`` (float32,
+    the 16-bit parameters'; a float32 parameter is its own master) and, with
+    32 bits, ``exp_avg`` and ``exp_avg_sq``, with 8 ``code_m``, ``code_r`` and
+    ``scales`` [blocks, 2].  ``state[p]`` has the same memory cut into
+    parameters.  They may be written in place, not replaced.
+
+    A parameter whose gradient is None is left alone, its step count too.  A
+    gradient that is not finite makes its block's moments not finite where they
+    are held in 8 bits; ``ops.grad_norm`` gives the multiplier that skips such
+    a step."""
+
+    def __init__(self, param_groups, betas: "tuple[float, float]" = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32, seed: int = 0):
+        b1, b2 = betas
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {betas}")
+        if not eps > 0.0:
+            raise ValueError(f"eps must be positive, got {eps}")
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        self.betas = (float(b1), float(b2))
+        self.eps = float(eps)
+        self.state_bits = state_bits
+        self.seed = int(seed) & 0xFFFFFFFF
+        self.groups = []
+        for g in param_groups:
+            params = [p for p in g["params"] if p.requires_grad]
+            self.groups.append({"params": params,
+                                "weight_decay": float(g.get("weight_decay", weight_decay))})
+        self._params = [p for g in self.groups for p in g["params"]]
+        if len({id(p) for p in self._params}) != len(self._params):
+            raise ValueError("a parameter appears twice")
+        for p in self._params:
+            if p.dtype not in _DTYPES:
+                raise ValueError(f"parameters must be float32, bfloat16 or "
+                                 f"float16, got {p.dtype}")
+            if p.device != self._params[0].device:
+                raise ValueError("parameters must be on one device")
+            if not _dense(p):
+                raise ValueError("parameters must be dense and without "
+                                 f"overlaps, got strides {p.stride()} of {tuple(p.shape)}")
+        self._grad_src = None
+        self._allocate()
+        self._make_plan()
+
+    def _allocate(self) -> None:
+        dev = self._params[0].device if self._params else torch.device("cpu")
+        places = sum(_padded(p.numel()) for p in self._params)
+        mplaces = sum(_padded(p.numel()) for p in self._params
+                      if p.dtype != torch.float32)
+
+        def zeros(n, dtype=torch.float32):
+            return torch.zeros(n, dtype=dtype, device=dev)
+
+        self._master = zeros(mplaces)
+        if self.state_bits == 32:
+            self._moments = [zeros(places), zeros(places)]
+        else:
+            self._moments = [zeros(places, torch.uint8),
+                             zeros(places, torch.uint8),
+                             zeros((places // _BLOCK, 2))]
+        self.state: dict[torch.nn.Parameter, dict] = {}
+        self._offsets, self._master_offsets, self._steps = [], [], []
+        at = mat = 0
+        for p in self._params:
+            n, pad = p.numel(), _padded(p.numel())
+            st = {}
+            if p.dtype != torch.float32:
+                st["master"] = self._master.as_strided(p.shape, p.stride(), mat)
+                st["master"].copy_(p.detach())
+            if self.state_bits == 32:
+                for k, f in zip(("exp_avg", "exp_avg_sq"), self._moments):
+                    st[k] = f.as_strided(p.shape, p.stride(), at)
+            else:
+                for k, f in zip(("code_m", "code_r"), self._moments):
+                    st[k] = f[at:at + pad]
+                st["scales"] = self._moments[2][at // _BLOCK:(at + pad) // _BLOCK]
+            self.state[p] = st
+            self._offsets.append(at)
+            self._master_offsets.append(mat if p.dtype != torch.float32 else -1)
+            self._steps.append(0)           # CPU path; the GPU has its own
+            at += pad
+            mat += pad if p.dtype != torch.float32 else 0
+
+    # -- flat states ---------------------------------------------------------
+    @property
+    def master(self) -> torch.Tensor:
+        return self._master
+
+    def _flat(self, bits: int, k: int) -> torch.Tensor:
+        if self.state_bits != bits:
+            raise AttributeError(f"the moments are held in {self.state_bits} bits")
+        return self._moments[k]
+
+    @property
+    def exp_avg(self) -> torch.Tensor:
+        return self._flat(32, 0)
+
+    @property
+    def exp_avg_sq(self) -> torch.Tensor:
+        return self._flat(32, 1)
+
+    @property
+    def code_m(self) -> torch.Tensor:
+        return self._flat(8, 0)
+
+    @property
+    def code_r(self) -> torch.Tensor:
+        return self._flat(8, 1)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._flat(8, 2)
+
+    def moments(self) -> "tuple[torch.Tensor, torch.Tensor]":
+        """The flat first and second moments: the float32 states themselves,
+        or the values that the 8-bit codes stand for, in new bfloat16 tensors."""
+        if self.state_bits == 32:
+            return self._moments[0], self._moments[1]
+        if self._master.is_cuda:
+            m, v = ext().adamw8_decode(*self._moments)
+            return m, v
+        m, r = reference.adamw8_decode(*self._moments)
+        return m.bfloat16(), (r * r).bfloat16()
+
+    # -- gradients read elsewhere than in .grad ------------------------------
+    # deferred-grad mode (reducer.defer): .grad is a fresh autograd tensor each
+    # step, and the reducer's gather lands it in the stable bucket views given
+    # here.  Without them a gradient that moved is seen, at the price of a new
+    # table in front of the step.
+    @property
+    def grad_src(self) -> "dict[torch.nn.Parameter, torch.Tensor] | None":
+        return self._grad_src
+
+    @grad_src.setter
+    def grad_src(self, views) -> None:
+        self._grad_src = views
+        if self._plan is not None:
+            none = torch.Tensor()
+            self._plan.set_grads([(views or {}).get(p, none) for p in self._params])
+
+    def _make_plan(self) -> None:
+        """The kernel's tables, on the GPU: made ahead of the first step, which
+        may be a captured one."""
+        self._plan = None
+        if self._params and self._params[0].is_cuda:
+            wd = [g["weight_decay"] for g in self.groups for _ in g["params"]]
+            self._plan = ext().AdamWPlan(self._params, wd, self._offsets,
+                                         self._master_offsets, self._master,
+                                         self._moments)
+            self._plan.set_steps(self._steps)
+            self.grad_src = self._grad_src
+
+    @torch.no_grad()
+    def step(self, lr, grad_scale: float = 1.0,
+             scale_t: "torch.Tensor | None" = None) -> None:
+        """``lr`` and ``scale_t`` as in ``SodSGD.step``: ``scale_t``, a float32
+        scalar on the parameters' device, is multiplied into ``grad_scale``
+        and skips the whole step where it is 0; ``lr`` may be a device float32
+        scalar, which a captured step reads anew on each replay."""
+        if not self._params:
+            return
+        if self._params[0].device != self._master.device:
+            raise RuntimeError("the parameters have moved to another device "
+                               "since the optimizer was made")
+        if self._plan is not None:
+            none = torch.Tensor()
+            on_gpu = isinstance(lr, torch.Tensor) and lr.is_cuda
+            self._plan.step(0.0 if on_gpu else float(lr),
+                            lr if on_gpu else none, *self.betas, self.eps,
+                            float(grad_scale),
+                            none if scale_t is None else scale_t, self.seed)
+            # weights just changed: re-transpose every cached dgrad w_t in
+            # one launch (sodkit/ops/conv.py _WtCache)
+            from . import conv as _conv
+            _conv._WtCache.refresh()
+            return
+        gs = torch.tensor(float(grad_scale))
+        if scale_t is not None:
+            if float(scale_t) == 0.0:
+                return
+            gs = gs * scale_t.to("cpu", torch.float32)
+        k = -1
+        for g in self.groups:
+            for p in g["params"]:
+                k += 1
+                grad = (self._grad_src or {}).get(p)
+                grad = p.grad if grad is None else grad
+                if grad is None:
+                    continue
+                if grad.layout != torch.strided or grad.shape != p.shape \
+                        or grad.dtype not in _DTYPES or grad.device != p.device:
+                    raise RuntimeError(
+                        f"the gradient of parameter {k} must be dense, of its "
+                        f"size, on its device and float32, bfloat16 or float16")
+                if p.numel() == 0:
+                    continue
+                grad = torch.empty_strided(p.shape, p.stride(), dtype=grad.dtype).copy_(grad)
+                self._steps[k] += 1
+                st = self.state[p]
+                w = _in_storage(st["master"] if "master" in st else p.data)
+                args = (float(lr), self._steps[k], self.betas, self.eps,
+                        g["weight_decay"], gs)
+                if self.state_bits == 32:
+                    reference.adamw_step(_in_storage(p.data), _in_storage(grad), w,
+                                         _in_storage(st["exp_avg"]),
+                                         _in_storage(st["exp_avg_sq"]), *args)
+                else:
+                    reference.adamw8_step(_in_storage(p.data), _in_storage(grad), w,
+                                          st["code_m"], st["code_r"], st["scales"],
+                                          *args, self.seed, k)
+
+    def set_step(self, step: int) -> None:
+        """Set every parameter's count of steps taken."""
+        if step < 0 or step >= 2 ** 31 - 1:
+            raise ValueError(f"step must lie in [0, 2^31 - 1), got {step}")
+        self._steps = [int(step)] * len(self._params)
+        if self._plan is not None:
+            self._plan.set_steps(self._steps)
+
+    # -- checkpointing (bitwise resume of optimizer state) -------------------
+    def state_dict(self) -> dict:
+        """References to the states, and each parameter's step count (which
+        waits for the GPU)."""
+        if self._plan is not None:
+            self._steps = self._plan.get_steps()
+        flat = [{**self.state[p], "step": t}
+                for p, t in zip(self._params, self._steps)]
+        return {"kind": "adamw", "state_bits": self.state_bits,
+                "betas": self.betas, "eps": self.eps, "seed": self.seed,
+                "param_state": flat,
+                "group_wd": [g["weight_decay"] for g in self.groups]}
+
+    def load_state_dict(self, sd: dict) -> None:
+        if sd.get("kind") != "adamw" or sd["state_bits"] != self.state_bits:
+            raise ValueError(
+                f"checkpoint holds the states of {sd.get('kind', 'sgd')}"
+                + (f" in {sd['state_bits']} bits" if "state_bits" in sd else "")
+                + f", not of adamw in {self.state_bits} bits")
+        saved = sd["param_state"]
+        if len(saved) != len(self._params) or len(sd["group_wd"]) != len(self.groups):
+            raise ValueError(f"checkpoint holds {len(saved)} parameters in "
+                             f"{len(sd['group_wd'])} groups, the optimizer "
+                             f"{len(self._params)} in {len(self.groups)}")
+        for k, (p, st) in enumerate(zip(self._params, saved)):
+            mine = self.state[p]
+            if set(st) - {"step"} != set(mine) or any(
+                    st[n].shape != mine[n].shape for n in mine):
+                raise ValueError(f"checkpoint's state of parameter {k} does "
+                                 f"not fit it")
+        self.betas, self.eps = tuple(sd["betas"]), sd["eps"]
+        self.seed = sd["seed"]
+        for p, st in zip(self._params, saved):
+            for n, t in self.state[p].items():
+                t.copy_(st[n])
+        self._steps = [int(st["step"]) for st in saved]
+        for g, wd in zip(self.groups, sd["group_wd"]):
+            g["weight_decay"] = wd
+        self._make_plan()
+
+    def params(self) -> Iterable[torch.nn.Parameter]:
+        for g in self.groups:
+            yield from g["params"]

@@ -207,3 +207,156 @@ def sgd_step(param, grad, master32, momentum_buf32, lr: float, momentum: float,
         g = momentum_buf32
     master32.add_(g, alpha=-lr)
     param.copy_(master32.to(param.dtype))
+
+
+# ---------------------------------------------------------------------------
+# Global gradient norm -> clip multiplier, overflow skip, dynamic loss scale.
+# ---------------------------------------------------------------------------
+
+_TINY32 = torch.finfo(torch.float32).tiny
+
+
+@torch.no_grad()
+def grad_norm(grads, prescale: float, max_norm: float, loss_scale=None,
+              good_steps=None, skips=None, growth_interval: int = 500):
+    for g in grads:
+        if g.device != grads[0].device or g.layout != torch.strided:
+            raise ValueError("gradients must be dense and on one device")
+        if g.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError(f"gradients must be float32, bfloat16 or "
+                             f"float16, got {g.dtype}")
+    total = sum(g.double().square().sum() for g in grads)
+    scale = (loss_scale.double() if loss_scale is not None
+             else torch.ones_like(total))
+    norm = (total.sqrt() * prescale / scale).float()
+    finite = torch.isfinite(norm)
+    clip = torch.ones_like(total)
+    if max_norm > 0:
+        clip = (max_norm / (norm.double() + 1e-6)).clamp(max=1.0)
+    # 0 means "skip the step": a finite norm never rounds to it
+    mult = torch.where(finite, (clip / scale).float().clamp(min=_TINY32),
+                       torch.zeros_like(norm))
+    if good_steps is not None:
+        good = torch.where(finite, good_steps + 1.0, torch.zeros_like(norm))
+        grow = good >= float(growth_interval)
+        up = torch.where(grow, (loss_scale * 2.0).clamp(max=65536.0),
+                         loss_scale)
+        loss_scale.copy_(torch.where(finite, up,
+                                     (loss_scale * 0.5).clamp(min=1.0)))
+        good_steps.copy_(torch.where(grow, torch.zeros_like(good), good))
+        skips += (~finite).float()
+    return norm, mult
+
+
+# ---------------------------------------------------------------------------
+# AdamW, moments in 32 or in 8 bits, on the flat elements of one tensor.  The
+# operations and their order are the kernel's (csrc/adamw.hip), each rounded
+# to float32 by itself.  `gs` is a float32 scalar tensor.
+# ---------------------------------------------------------------------------
+
+ADAMW_BLOCK = 256
+_M32 = 0xFFFFFFFF
+
+
+def _adamw_moments(grad, m, v, betas, gs):
+    b1, b2 = betas
+    g = grad.float() * gs
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + (g * (1 - b2)) * g
+    return m, v
+
+
+def _root(v):
+    """The float32 root to the last bit, which torch's own on the CPU is not (one
+    in six is a unit off): the root in 64 bits, rounded."""
+    return v.double().sqrt().float()
+
+
+def _adamw_weight(param, w, m, r, lr, step, betas, eps, weight_decay):
+    b1, b2 = betas
+    rate = lr / (1 - b1 ** step)
+    den = r * (1 / math.sqrt(1 - b2 ** step)) + eps
+    new = w * (1 - lr * weight_decay) - (m / den) * rate
+    w.copy_(new)
+    if param.dtype == torch.float16:      # saturates, as every kernel's cast
+        big = torch.finfo(torch.float16).max
+        new = new.clamp(-big, big)
+    param.copy_(new)
+
+
+@torch.no_grad()
+def adamw_step(param, grad, w, exp_avg, exp_avg_sq, lr: float, step: int,
+               betas, eps: float, weight_decay: float, gs):
+    m, v = _adamw_moments(grad, exp_avg, exp_avg_sq, betas, gs)
+    exp_avg.copy_(m)
+    exp_avg_sq.copy_(v)
+    _adamw_weight(param, w, m, _root(v), lr, step, betas, eps, weight_decay)
+
+
+def _mix32(h):
+    """The finalizer of MurmurHash3 (Appleby, public domain) on int64 tensors
+    or ints that hold 32 bits."""
+    h = h ^ (h >> 16)
+    h = (h * 0x85EBCA6B) & _M32
+    h = h ^ (h >> 13)
+    h = (h * 0xC2B2AE35) & _M32
+    return h ^ (h >> 16)
+
+
+def adamw8_noise(places: int, seed: int, step: int, tensor: int,
+                 first: int = 0):
+    """The 32 random bits of each element from `first` on: the upper half rounds
+    m, the lower half r."""
+    key = _mix32((seed + step * 0x9E3779B9) & _M32)
+    key = _mix32((key + tensor) & _M32)
+    i = torch.arange(first, first + places, dtype=torch.int64)
+    key = _mix32((key + (i >> 32)) & _M32)
+    return _mix32(((i & _M32) + key) & _M32)
+
+
+def _adamw8_grid(code, bias: int, shift: int):
+    bits = torch.where(code > 0, (code + bias) << shift, torch.zeros_like(code))
+    return bits.view(torch.float32)
+
+
+def adamw8_decode(code_m, code_r, scales):
+    """(m, r) in float32: the values of the codes of whole blocks."""
+    cm, cr = code_m.to(torch.int32), code_r.to(torch.int32)
+    m = _adamw8_grid(cm & 127, 889, 20).view(-1, ADAMW_BLOCK) * scales[:, :1]
+    m = torch.where((cm > 127).view_as(m), -m, m)
+    r = _adamw8_grid(cr, 1777, 19).view(-1, ADAMW_BLOCK) * scales[:, 1:]
+    return m.reshape(-1), r.reshape(-1)
+
+
+def adamw8_encode(m, r, noise):
+    """(code_m, code_r, scales) of whole blocks, rounded by the noise."""
+    def codes(x, top, noise16, bias, shift):
+        inv = 1.0 / top.clamp(min=2.0 ** -100)
+        bits = (x * inv).view(torch.int32) & 0x7FFFFFFF
+        bits = bits.clamp(max=0x3F800000)
+        return ((bits + (noise16 << (shift - 16))) >> shift) - bias
+
+    m, r = m.view(-1, ADAMW_BLOCK), r.view(-1, ADAMW_BLOCK)
+    noise = noise.view(-1, ADAMW_BLOCK)
+    sm, sr = m.abs().amax(1, keepdim=True), r.amax(1, keepdim=True)
+    cm = codes(m.abs(), sm, (noise >> 16).to(torch.int32), 889, 20).clamp(min=0)
+    cm = torch.where((m < 0) & (cm > 0), cm + 128, cm)
+    cr = codes(r, sr, (noise & 0xFFFF).to(torch.int32), 1777, 19).clamp(min=1)
+    cr = torch.where(r > 0, cr, torch.zeros_like(cr))
+    return (cm.to(torch.uint8).view(-1), cr.to(torch.uint8).view(-1),
+            torch.cat([sm, sr], 1))
+
+
+@torch.no_grad()
+def adamw8_step(param, grad, w, code_m, code_r, scales, lr: float, step: int,
+                betas, eps: float, weight_decay: float, gs, seed: int,
+                tensor: int):
+    n, places = param.numel(), code_m.numel()
+    m, r = adamw8_decode(code_m, code_r, scales)
+    m, v = _adamw_moments(F.pad(grad.float(), (0, places - n)), m, r * r,
+                          betas, gs)
+    r = _root(v)
+    _adamw_weight(param, w, m[:n], r[:n], lr, step, betas, eps, weight_decay)
+    for dst, src in zip((code_m, code_r, scales),
+                        adamw8_encode(m, r, adamw8_noise(places, seed, step, tensor))):
+        dst.copy_(src)

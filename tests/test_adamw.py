@@ -1,0 +1,393 @@
+"""SodAdamW (moments in 32 and in 8 bits) and grad_norm on the CPU: against
+their definitions in 64 bits, torch's own AdamW, and what they refuse."""
+
+import math
+
+import pytest
+import torch
+
+from adamw_oracle import check, decode64, level, param_bound, step64
+from sodkit.config import make_config
+from sodkit.engine import Solver
+from sodkit.ops import SodAdamW, SodSGD, grad_norm, reference
+
+HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, wd=0.1)
+
+
+def make(n, dtype=torch.float32, bits=32, seed=0, **kw):
+    g = torch.Generator().manual_seed(seed)
+    p = torch.nn.Parameter(torch.randn(n, generator=g).to(dtype))
+    opt = SodAdamW([{"params": [p], "weight_decay": HYPER["wd"]}],
+                   betas=HYPER["betas"], eps=HYPER["eps"], state_bits=bits,
+                   seed=5, **kw)
+    return p, opt, g
+
+
+@pytest.mark.parametrize("n", [1, 3, 255, 256, 257, 1000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_step_against_64_bits(n, dtype):
+    p, opt, gen = make(n, dtype)
+    st = opt.state[p]
+    for t in range(1, 4):
+        p.grad = (torch.randn(n, generator=gen) * 10.0 ** (t - 2)).to(dtype)
+        w = st["master"] if "master" in st else p.detach()
+        w1, m1, v1, em, ev, ew = step64(
+            w.double(), p.grad.double(), st["exp_avg"].double(),
+            st["exp_avg_sq"].double(), t, gs=0.25, **HYPER)
+        opt.step(HYPER["lr"], 0.25)
+        check(st["exp_avg"], m1, em, "m")
+        check(st["exp_avg_sq"], v1, ev, "v")
+        if "master" in st:
+            check(st["master"], w1, ew, "master")
+        check(p.detach(), w1, param_bound(w1, ew, dtype), "param")
+
+
+def test_matches_torch_adamw():
+    """Ten steps of torch.optim.AdamW: each may differ by the roundings of the
+    weight (4 of 2^-24 relative) and of the update (24, of at most 1.2 lr)."""
+    p, opt, gen = make(500)
+    q = torch.nn.Parameter(p.detach().clone())
+    ref = torch.optim.AdamW([q], lr=HYPER["lr"], betas=HYPER["betas"],
+                            eps=HYPER["eps"], weight_decay=HYPER["wd"])
+    for _ in range(10):
+        p.grad = torch.randn(500, generator=gen)
+        q.grad = p.grad.clone()
+        opt.step(HYPER["lr"])
+        ref.step()
+    bound = 10 * 2.0 ** -24 * (4 * (q.abs() + 0.1) + 24 * 2 * HYPER["lr"])
+    assert ((p - q).abs() <= bound).all()
+
+
+def test_groups_scale_and_skip():
+    ps = [torch.nn.Parameter(torch.ones(5)) for _ in range(3)]
+    opt = SodAdamW([{"params": ps[:1], "weight_decay": 0.5},
+                    {"params": ps[1:]}], weight_decay=0.0)
+    for p in ps[:2]:
+        p.grad = torch.zeros(5)
+    opt.step(0.1)                       # no gradient: decay alone, or nothing
+    assert torch.equal(ps[0], torch.full((5,), 1.0) * (1 - 0.1 * 0.5))
+    assert torch.equal(ps[1], torch.ones(5))
+    assert [s["step"] for s in opt.state_dict()["param_state"]] == [1, 1, 0]
+    ps[2].grad = torch.full((5,), 3.0)
+    opt.step(0.1, scale_t=torch.tensor(0.0))
+    assert [s["step"] for s in opt.state_dict()["param_state"]] == [1, 1, 0]
+    assert torch.equal(ps[2], torch.ones(5))
+    a = ps[2].detach().clone()
+    opt.step(0.1, 0.5, scale_t=torch.tensor(0.25))
+    want = step64(a.double(), torch.full((5,), 3.0).double(),
+                  torch.zeros(5).double(), torch.zeros(5).double(), 1, 0.1,
+                  (0.9, 0.999), 1e-8, 0.0, 0.125)
+    check(ps[2].detach(), want[0], want[5], "scaled")
+
+
+def test_strided_parameters_and_gradients():
+    """Parameters in another order than row by row, gradients in either."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 5, 4, 3, generator=g)
+    dense = torch.nn.Parameter(x.clone())
+    last = torch.nn.Parameter(x.clone().contiguous(memory_format=torch.channels_last))
+    for bits in (32, 8):
+        opts = [SodAdamW([{"params": [p]}], state_bits=bits) for p in (dense, last)]
+        assert opts[1].state[last].get("exp_avg", last).stride() == last.stride()
+        for grad_last in (False, True):
+            gr = torch.randn(6, 5, 4, 3, generator=g)
+            if grad_last:
+                gr = gr.contiguous(memory_format=torch.channels_last)
+            dense.grad, last.grad = gr.clone(), gr.clone()
+            for o in opts:
+                o.step(0.01)
+        if bits == 32:
+            assert torch.equal(dense, last)
+
+
+# ------------------------------------------------------------------ 8 bits
+
+def test_codes_are_levels():
+    """Every code is the value it stands for, to the bit."""
+    c = torch.arange(256, dtype=torch.uint8)
+    m, r = reference.adamw8_decode(c, c, torch.ones(1, 2))
+    m64, r64 = decode64(c.int(), c.int(), torch.ones(1, 2))
+    assert torch.equal(m.double(), m64) and torch.equal(r.double(), r64)
+    assert m[127] == 1 and m[255] == -1 and r[255] == 1 and r[0] == 0
+    assert (r[1:].diff() > 0).all()
+
+
+def test_rounding_keeps_the_mean():
+    """Over all 65536 noises a value's mean is itself, to the 16 bits of the noise:
+    the bits below them (4 of m's 20 cut, 3 of r's 19) are lost, under one in
+    65536 of a code step, 1/8 and 1/16 of the value at most."""
+    noise = torch.arange(65536, dtype=torch.int64)
+    for x in (1.0, 0.7301, 0.3, 0.0123, 1.7e-3, 4.4e-5):
+        for which, steps in ((0, 8), (1, 16)):
+            v = torch.full((65536, 256), x)
+            v[:, 0] = 1.0                   # the block's largest
+            n = (noise << 16 if which == 0 else noise).view(-1, 1).expand(-1, 256)
+            args = (v, torch.zeros_like(v)) if which == 0 else (torch.zeros_like(v), v)
+            got = torch.stack(reference.adamw8_decode(*reference.adamw8_encode(
+                *(a.reshape(-1) for a in args), n.reshape(-1))))[which]
+            mean = got.double().view(-1, 256)[:, 1].mean().item()
+            want = float(torch.tensor(x).double())
+            assert abs(mean - want) <= want / steps / 65536 * 1.001, (x, which)
+
+
+def test_r_never_rounds_to_zero():
+    r = torch.full((256,), 1e-30)
+    r[0], r[1] = 1.0, 0.0
+    for n in (0, 0xFFFFFFFF):
+        _, code, _ = reference.adamw8_encode(torch.zeros(256), r,
+                                             torch.full((256,), n, dtype=torch.int64))
+        assert code[0] == 255 and code[1] == 0 and (code[2:] == 1).all()
+
+
+@pytest.mark.parametrize("n", [1, 255, 256, 257, 1000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step8_against_64_bits(n, dtype):
+    """The weight goes by the moments before they are rounded; the codes lie
+    within a step, 1/8 of m and 1/16 of r, of them."""
+    p, opt, gen = make(n, dtype, bits=8)
+    st = opt.state[p]
+    for t in range(1, 4):
+        p.grad = (torch.randn(n, generator=gen) * 10.0 ** (t - 2)).to(dtype)
+        m0, r0 = decode64(st["code_m"].int(), st["code_r"].int(), st["scales"])
+        w = st["master"] if "master" in st else p.detach()
+        w1, m1, v1, em, ev, ew = step64(w.double(), p.grad.double(), m0[:n],
+                                        r0[:n] ** 2, t, gs=1.0, **HYPER)
+        # the old moments' own roundings: their scale's product, r's square
+        ew = ew * 2
+        opt.step(HYPER["lr"])
+        check(p.detach(), w1, param_bound(w1, ew, dtype), "param")
+        m, r = decode64(st["code_m"].int(), st["code_r"].int(), st["scales"])
+        blk = torch.arange(n) // 256
+        floor = st["scales"].double()[blk] * 2.0 ** -15
+        check(m[:n], m1, m1.abs() / 8 + floor[:, 0] + em, "m")
+        check(r[:n], v1.sqrt(), v1.sqrt() / 16 * (1 + 1e-5) + floor[:, 1], "r")
+        assert (st["code_m"][n:] == 0).all() and (st["code_r"][n:] == 0).all()
+
+
+def test_r_follows_a_change():
+    """r of elements whose gradients grow a hundredfold follows them, though most
+    steps move it by far less than half a code step: the rounding keeps the
+    mean, and over 256 elements that each lie within a code step or two (6 % of
+    r, 13 % of v) the mean is good to a few percent."""
+    p, opt, _ = make(512, bits=8)
+    small = torch.ones(512)
+    small[::2] = 0.01                       # the other half sets the scales
+    for _ in range(200):
+        p.grad = small
+        opt.step(0.0)
+    p.grad = torch.ones(512)
+    for _ in range(300):
+        opt.step(0.0)
+    _, v = opt.moments()
+    want = 0.001 * sum(0.999 ** i * (1.0 if i < 300 else 1e-4) for i in range(500))
+    got = v.float()[::2].mean().item()
+    assert abs(got / want - 1) < 0.1, (got, want)
+
+
+def test_non_finite_gradient_is_loud():
+    p, opt, _ = make(512, bits=8)
+    p.grad = torch.zeros(512)
+    p.grad[300] = math.nan
+    opt.step(0.1)
+    s = opt.scales
+    assert torch.isfinite(s[0]).all() and torch.isnan(s[1]).all()
+    m, v = opt.moments()
+    assert torch.isnan(m[256:512]).all() and torch.isfinite(m[:256]).all()
+    p.grad[300] = math.inf
+    opt2 = SodAdamW([{"params": [p]}], state_bits=8)
+    opt2.step(0.1)
+    assert not torch.isfinite(opt2.scales[1]).any()
+
+
+def test_noise_past_32_bits():
+    """Elements 2^32 apart have other noise, tensors and steps too."""
+    a = reference.adamw8_noise(4, 1, 1, 0)
+    assert not torch.equal(a, reference.adamw8_noise(4, 1, 2, 0))
+    assert not torch.equal(a, reference.adamw8_noise(4, 1, 1, 1))
+    far = reference.adamw8_noise(4, 1, 1, 0, first=2 ** 32)
+    assert not torch.equal(a, far)
+    assert torch.equal(reference.adamw8_noise(6, 1, 1, 0, first=2 ** 32 - 2)[2:], far)
+
+
+# ------------------------------------------------------------------ state
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_resume_is_bitwise(bits, tmp_path):
+    p, opt, gen = make(700, torch.bfloat16, bits)
+    for _ in range(3):
+        p.grad = torch.randn(700, generator=gen).bfloat16()
+        opt.step(0.01)
+    torch.save(opt.state_dict(), tmp_path / "o.pt")
+    q = torch.nn.Parameter(p.detach().clone())
+    other = SodAdamW([{"params": [q], "weight_decay": 0.0}], state_bits=bits, seed=77)
+    other.load_state_dict(torch.load(tmp_path / "o.pt", weights_only=True))
+    for _ in range(2):
+        p.grad = torch.randn(700, generator=gen).bfloat16()
+        q.grad = p.grad.clone()
+        opt.step(0.01)
+        other.step(0.01)
+    assert torch.equal(p, q) and torch.equal(opt.master, other.master)
+    for a, b in zip(opt.moments(), other.moments()):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    p = torch.nn.Parameter(torch.ones(4))
+    ok = [{"params": [p]}]
+    for kw in (dict(betas=(1.0, 0.9)), dict(betas=(-0.1, 0.9)), dict(eps=0.0),
+               dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            SodAdamW(ok, **kw)
+    with pytest.raises(ValueError, match="twice"):
+        SodAdamW([{"params": [p, p]}])
+    with pytest.raises(ValueError, match="float"):
+        SodAdamW([{"params": [torch.nn.Parameter(torch.ones(4).double())]}])
+    with pytest.raises(ValueError, match="dense"):
+        SodAdamW([{"params": [torch.nn.Parameter(torch.ones(8)[::2])]}])
+    with pytest.raises(ValueError, match="dense"):
+        SodAdamW([{"params": [torch.nn.Parameter(torch.ones(1).expand(4))]}])
+    opt = SodAdamW(ok)
+    with pytest.raises(AttributeError):
+        opt.code_m
+    with pytest.raises(ValueError):
+        opt.set_step(-1)
+    opt.grad_src = {p: torch.ones(5)}
+    with pytest.raises(RuntimeError, match="size"):
+        opt.step(0.1)
+    sgd = SodSGD(ok)
+    with pytest.raises(ValueError, match="sgd"):
+        opt.load_state_dict(sgd.state_dict())
+    with pytest.raises(ValueError, match="32 bits"):
+        SodAdamW(ok, state_bits=8).load_state_dict(opt.state_dict())
+    two = SodAdamW([{"params": [p, torch.nn.Parameter(torch.ones(4))]}])
+    with pytest.raises(ValueError, match="parameters"):
+        two.load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError, match="fit"):
+        SodAdamW([{"params": [torch.nn.Parameter(torch.ones(5))]}]).load_state_dict(
+            opt.state_dict())
+    assert SodAdamW([]).step(0.1) is None
+
+
+def test_native_refusals():
+    """The extension's own checks, which a GPU call would reach."""
+    from sodkit import _C
+    none = torch.Tensor()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _C.grad_norm([], 1.0, 0.0, none, none, none, 500.0)
+    with pytest.raises(RuntimeError, match="GPU"):
+        _C.grad_norm([torch.ones(3)], 1.0, 0.0, none, none, none, 500.0)
+    with pytest.raises(RuntimeError):
+        _C.AdamWPlan([torch.ones(3)], [0.0], [0], [-1], none, [none, none])
+    with pytest.raises(RuntimeError):
+        _C.adamw8_decode(torch.zeros(256, dtype=torch.uint8),
+                         torch.zeros(256, dtype=torch.uint8), torch.zeros(1, 2))
+
+
+# ------------------------------------------------------------------ the norm
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_grad_norm(dtype):
+    """The sum is in 64 bits, so only the two results' own roundings count."""
+    g = torch.Generator().manual_seed(0)
+    grads = [torch.randn(n, generator=g).to(dtype) for n in (0, 1, 7, 1000)]
+    grads.append(torch.randn(33, 9, generator=g).t())
+    n64 = math.sqrt(sum((x.double() ** 2).sum().item() for x in grads)) * 0.5
+    norm, mult = grad_norm(grads, prescale=0.5)
+    assert abs(norm.item() - n64) <= 2.0 ** -23 * n64 and mult.item() == 1.0
+    norm, mult = grad_norm(grads, prescale=0.5, max_norm=0.1)
+    assert abs(mult.item() - 0.1 / (n64 + 1e-6)) <= 2.0 ** -22 * mult.item()
+    _, mult = grad_norm(grads, max_norm=1e9, loss_scale=torch.tensor(4.0))
+    assert mult.item() == 0.25
+
+
+def test_grad_norm_range():
+    """Squares past float32's range are no overflow, and a tiny multiplier is
+    no skip."""
+    norm, mult = grad_norm([torch.full((4,), 1e38)], max_norm=1e-6)
+    assert abs(norm.item() / 2e38 - 1) < 1e-6 and mult.item() > 0
+    for bad in (math.inf, -math.inf, math.nan):
+        norm, mult = grad_norm([torch.tensor([1.0, bad])], max_norm=1.0)
+        assert not math.isfinite(norm.item()) and mult.item() == 0.0
+    norm, mult = grad_norm([torch.zeros(0)], max_norm=1.0)
+    assert norm.item() == 0.0 and mult.item() == 1.0
+
+
+def test_grad_norm_scaler():
+    scale, good, skips = torch.tensor(64.0), torch.tensor(0.0), torch.tensor(0.0)
+    kw = dict(loss_scale=scale, good_steps=good, skips=skips, growth_interval=2)
+    fine, bad = [torch.ones(3)], [torch.tensor([math.inf])]
+    assert grad_norm(fine, **kw)[1].item() == 1 / 64
+    assert (scale.item(), good.item()) == (64.0, 1.0)
+    assert grad_norm(fine, **kw)[1].item() == 1 / 64     # by the scale before
+    assert (scale.item(), good.item()) == (128.0, 0.0)
+    assert grad_norm(bad, **kw)[1].item() == 0.0
+    assert (scale.item(), good.item(), skips.item()) == (64.0, 0.0, 1.0)
+    scale.fill_(1.0)
+    grad_norm(bad, **kw)
+    assert scale.item() == 1.0 and skips.item() == 2.0
+    scale.fill_(65536.0)
+    good.fill_(1.0)
+    grad_norm(fine, **kw)
+    assert scale.item() == 65536.0
+
+
+def test_grad_norm_refusals():
+    with pytest.raises(ValueError):
+        grad_norm([])
+    with pytest.raises(ValueError):
+        grad_norm([torch.ones(3).double()])
+    with pytest.raises(ValueError):
+        grad_norm([torch.ones(3)], good_steps=torch.tensor(0.0))
+    with pytest.raises(ValueError):
+        grad_norm([torch.ones(3)], good_steps=torch.tensor(0.0),
+                  skips=torch.tensor(0.0))
+    with pytest.raises(ValueError):
+        grad_norm([torch.ones(3)], growth_interval=0)
+
+
+# ------------------------------------------------------------------ the solver
+
+def _solver(tmp_path, **kw):
+    return Solver(make_config("cpu_plumbing", output_root=str(tmp_path), size=48,
+                              train_samples=4, val_samples=2, epoch_num=1,
+                              num_workers=0, log_interval=1, optimizer="adamw",
+                              lr=1e-3, **kw))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_solver_trains_and_resumes(tmp_path, bits):
+    s = _solver(tmp_path, adam_state_bits=bits, grad_clip=1.0)
+    assert isinstance(s.optimizer, SodAdamW) and s.optimizer.state_bits == bits
+    before = [p.detach().clone() for p in s.model.parameters()]
+    s.train()
+    assert any(not torch.equal(a, b) for a, b in zip(before, s.model.parameters()))
+    r = _solver(tmp_path, adam_state_bits=bits, resume=True)
+    r.train()                                   # loads; no epoch is left
+    for a, b in zip(s.optimizer.state_dict()["param_state"],
+                    r.optimizer.state_dict()["param_state"]):
+        assert a["step"] == b["step"] == 2
+        for k in a:
+            assert k == "step" or torch.equal(a[k], b[k])
+    with pytest.raises(ValueError, match="checkpoint"):
+        _solver(tmp_path, adam_state_bits=40 - bits, resume=True).train()
+
+
+def test_solver_device_scaler_state(tmp_path):
+    """The device scaler with adamw moves as the one with sgd does."""
+    s = _solver(tmp_path)
+    s.dynamic_scale = s._use_device_scaler = True
+    s._growth_interval = 2
+    s._scale_t, s._good_t, s._skips_t = torch.tensor(64.0), torch.zeros(()), torch.zeros(())
+    for b in s.reducer.buckets:
+        b.flat.fill_(1.0)
+    assert s._device_clip_and_scale().item() == 1 / 64
+    assert s._device_clip_and_scale().item() == 1 / 64
+    assert s._scale_t.item() == 128.0
+    s.reducer.buckets[0].flat[0] = float("inf")
+    assert s._device_clip_and_scale().item() == 0.0
+    assert (s._scale_t.item(), s._skips_t.item()) == (64.0, 1.0)
+
+
+def test_unknown_optimizer(tmp_path):
+    with pytest.raises(ValueError, match="optimizer"):
+        Solver(make_config("cpu_plumbing", output_root=str(tmp_path), optimizer="adam"))
