@@ -27,7 +27,8 @@
 namespace sodkit {
 namespace aw {
 
-constexpr int CHUNK = 4096;     // elements of a workgroup
+constexpr int CHUNK32 = 1024;   // elements of a workgroup, moments in 32 bits
+constexpr int CHUNK8 = 2048;    // and in 8
 constexpr int BLOCK = 256;      // elements of an 8-bit block; tensors start at
 //                                 multiples of it in the states
 constexpr int ROWS = 160;       // table rows in one kernel's arguments
@@ -71,55 +72,59 @@ struct Args {
     unsigned seed;
 };
 
+// Addresses out of a table: said to be global memory, else they are loaded
+// through the flat path, which takes the LDS counter too.
+#define SOD_GLOBAL __attribute__((address_space(1)))
+template <typename T>
+SOD_DEVINL SOD_GLOBAL T *global_ptr(const void *p) {
+    return (SOD_GLOBAL T *)(unsigned long)p;
+}
+
 template <typename T> struct Vec4;  // 4 elements at any element's address
 template <> struct Vec4<float> {
+    typedef float elem;
     typedef float type __attribute__((ext_vector_type(4), aligned(4)));
 };
 template <> struct Vec4<__hip_bfloat16> {
+    typedef short elem;
     typedef short type __attribute__((ext_vector_type(4), aligned(2)));
 };
 template <> struct Vec4<__half> {
+    typedef short elem;
     typedef short type __attribute__((ext_vector_type(4), aligned(2)));
 };
 
+// A quad of a parameter or gradient.  FULL: all four lie in the tensor, and the
+// load is the only thing that happens (converted where it is used, so that
+// nothing waits for it between this and the next load).
+template <typename T, bool FULL>
+SOD_DEVINL typename Vec4<T>::type load4(const SOD_GLOBAL T *p, long n) {
+    using V = typename Vec4<T>::type;
+    if (FULL || n >= 4) return *(const SOD_GLOBAL V *)p;
+    V r = {};
+    for (int e = 0; e < 3; ++e)
+        if (e < n) r[e] = ((const SOD_GLOBAL typename Vec4<T>::elem *)p)[e];
+    return r;
+}
+SOD_DEVINL f32x4 to_f32(Vec4<float>::type v, float) { return v; }
 template <typename T>
-SOD_DEVINL f32x4 load4(const T *p, long n) {
-    f32x4 r = {0.f, 0.f, 0.f, 0.f};
-    if (n >= 4) {
-        auto v = *reinterpret_cast<const typename Vec4<T>::type *>(p);
+SOD_DEVINL f32x4 to_f32(typename Vec4<T>::type v, T) {
+    f32x4 r;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (sizeof(T) == 4) r[e] = v[e];
-            else r[e] = s16_as_f32<T>(v[e]);
-        }
-    } else {
-        for (int e = 0; e < 3; ++e)
-            if (e < n) r[e] = ElemTraits<T>::to_f32(p[e]);
-    }
+    for (int e = 0; e < 4; ++e) r[e] = s16_as_f32<T>(v[e]);
     return r;
 }
 
-template <typename T>
-SOD_DEVINL void store4(T *p, long n, f32x4 r) {
-    if (n >= 4) {
-        typename Vec4<T>::type v;
-        if constexpr (sizeof(T) == 4) v = r;
-        else v = pack4<T>(r);
-        *reinterpret_cast<typename Vec4<T>::type *>(p) = v;
-    } else {
+template <typename T, bool FULL>
+SOD_DEVINL void store4(SOD_GLOBAL T *p, long n, f32x4 r) {
+    using V = typename Vec4<T>::type;
+    V v;
+    if constexpr (sizeof(T) == 4) v = r;
+    else v = pack4<T>(r);
+    if (FULL || n >= 4) __builtin_nontemporal_store(v, (SOD_GLOBAL V *)p);
+    else
         for (int e = 0; e < 3; ++e)
-            if (e < n) p[e] = ElemTraits<T>::from_f32(r[e]);
-    }
-}
-
-// b^t by squaring; b^t in float64 to a few units of its last place
-SOD_DEVINL double ipow(double b, unsigned t) {
-    double r = 1.0;
-    for (; t; t >>= 1) {
-        if (t & 1) r *= b;
-        b *= b;
-    }
-    return r;
+            if (e < n) ((SOD_GLOBAL typename Vec4<T>::elem *)p)[e] = v[e];
 }
 
 // The scalars of a step, equal over a workgroup.
@@ -134,18 +139,32 @@ SOD_DEVINL unsigned mix32(unsigned h) {
     return h ^ (h >> 16);
 }
 
+// One wave works them out for its workgroup, another one from workgroup to
+// workgroup, as its SIMD has the time to give; its lanes 0 and 1 go through the
+// same float64 operations with b1 and b2: the power by squaring (a few units
+// of its last place, which rounding to float32 takes up), root and quotient.
 SOD_DEVINL Scalars step_scalars(const Args &a, double wd, int tensor, long off) {
     __shared__ Scalars sh;
-    if (threadIdx.x == 0) {
+    if ((threadIdx.x >> 6) == (blockIdx.x & 3)) {
+        const bool second = threadIdx.x & 1;
         unsigned t = (unsigned)a.steps[blockIdx.x] + 1u;
-        a.steps[blockIdx.x] = (int)t;
         double lr = a.lr_t ? (double)*a.lr_t : a.lr;
-        sh.rate = (float)(lr / (1.0 - ipow(a.b1, t)));
-        sh.rbc2 = (float)(1.0 / sqrt(1.0 - ipow(a.b2, t)));
-        sh.keep = (float)(1.0 - lr * wd);
-        unsigned k = mix32(a.seed + t * 0x9E3779B9u);
-        k = mix32(k + (unsigned)tensor);
-        sh.key = mix32(k + (unsigned)(off >> 32));
+        double b = second ? a.b2 : a.b1, p = 1.0;
+        for (unsigned k = t; k; k >>= 1) {
+            if (k & 1) p *= b;
+            b *= b;
+        }
+        double bc = 1.0 - p;
+        float q = (float)((second ? 1.0 : lr) / (second ? sqrt(bc) : bc));
+        if ((threadIdx.x & 63) == 1) sh.rbc2 = q;
+        if ((threadIdx.x & 63) == 0) {
+            a.steps[blockIdx.x] = (int)t;
+            sh.rate = q;
+            sh.keep = (float)(1.0 - lr * wd);
+            unsigned k = mix32(a.seed + t * 0x9E3779B9u);
+            k = mix32(k + (unsigned)tensor);
+            sh.key = mix32(k + (unsigned)(off >> 32));
+        }
     }
     __syncthreads();
     return sh;
@@ -158,34 +177,39 @@ SOD_DEVINL float moved(float w, float m, float r, float eps, const Scalars &s) {
 
 // -------------------------------------------------------------- 32 bits
 
-template <typename P, typename G>
-SOD_DEVINL void chunk32(const Args &a, const Info &I, const Row &R, long off,
-                        float *m_, float *v_, float gs, const Scalars &s) {
-    P *p = reinterpret_cast<P *>(R.param);
-    const G *g_ = reinterpret_cast<const G *>(R.grad);
-    long end = min(off + (long)CHUNK, I.numel);
-    for (long i = off + threadIdx.x * 4; i < end; i += 1024) {
-        long n = I.numel - i;
-        f32x4 g = load4(g_ + i, n);
-        f32x4 m = *reinterpret_cast<f32x4 *>(m_ + I.state + i);
-        f32x4 v = *reinterpret_cast<f32x4 *>(v_ + I.state + i);
-        f32x4 w;
-        if constexpr (sizeof(P) == 4) w = load4(p + i, n);
-        else w = *reinterpret_cast<f32x4 *>(a.master + I.master + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x = g[e] * gs;
-            m[e] = a.fb1 * m[e] + a.fc1 * x;
-            v[e] = a.fb2 * v[e] + (a.fc2 * x) * x;
-            w[e] = moved(w[e], m[e], sqrtf(v[e]), a.eps, s);
-        }
-        // the states are padded past a tensor's end, its gradient reads 0 there
-        *reinterpret_cast<f32x4 *>(m_ + I.state + i) = m;
-        *reinterpret_cast<f32x4 *>(v_ + I.state + i) = v;
-        if constexpr (sizeof(P) != 4)
-            *reinterpret_cast<f32x4 *>(a.master + I.master + i) = w;
-        store4(p + i, n, w);
+template <typename P, typename G, bool FULL>
+SOD_DEVINL void step32(const Args &a, const Info &I, const Row &R, int tensor,
+                       long off, float *m_, float *v_, float gs) {
+    Scalars s = step_scalars(a, I.wd, tensor, off);
+    long i = off + threadIdx.x * 4, n = I.numel - i;
+    SOD_GLOBAL P *p = global_ptr<P>(R.param) + i;
+    const SOD_GLOBAL G *g_ = global_ptr<G>(R.grad) + i;
+    f32x4 *mp = reinterpret_cast<f32x4 *>(m_ + I.state + i);
+    f32x4 *vp = reinterpret_cast<f32x4 *>(v_ + I.state + i);
+    f32x4 *wp = reinterpret_cast<f32x4 *>(a.master + I.master + i);
+    typename Vec4<G>::type gq;
+    f32x4 m, v, w;
+    if (FULL || n > 0) {
+        gq = load4<G, FULL>(g_, n);
+        m = __builtin_nontemporal_load(mp);
+        v = __builtin_nontemporal_load(vp);
+        if constexpr (sizeof(P) == 4) w = load4<P, FULL>(p, n);
+        else w = __builtin_nontemporal_load(wp);
     }
+    if (!FULL && n <= 0) return;
+    f32x4 g = to_f32(gq, G());
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x = g[e] * gs;
+        m[e] = a.fb1 * m[e] + a.fc1 * x;
+        v[e] = a.fb2 * v[e] + (a.fc2 * x) * x;
+        w[e] = moved(w[e], m[e], sqrtf(v[e]), a.eps, s);
+    }
+    // the gap behind a tensor's end read gradients of 0 and stays 0
+    __builtin_nontemporal_store(m, mp);
+    __builtin_nontemporal_store(v, vp);
+    if constexpr (sizeof(P) != 4) __builtin_nontemporal_store(w, wp);
+    store4<P, FULL>(p, n, w);
 }
 
 // call f with a tag of the parameter's and of the gradient's type
@@ -224,11 +248,14 @@ adamw32_kernel(const Args a, float *__restrict__ m, float *__restrict__ v) {
     Info I = a.info[c.x];
     Row R = a.rows[c.x];
     if (R.grad == nullptr || !scaled(a, gs)) return;
-    long off = (long)c.y * CHUNK;
-    Scalars s = step_scalars(a, I.wd, c.x, off);
     by_types(I.dtype, R.grad_dtype, [&](auto p, auto g) {
-        chunk32<typename decltype(p)::type, typename decltype(g)::type>(
-            a, I, R, off, m, v, gs, s);
+        using P = typename decltype(p)::type;
+        using G = typename decltype(g)::type;
+        long off = (long)c.y * CHUNK32;
+        if (off + CHUNK32 <= I.numel)
+            step32<P, G, true>(a, I, R, c.x, off, m, v, gs);
+        else
+            step32<P, G, false>(a, I, R, c.x, off, m, v, gs);
     });
 }
 
@@ -253,123 +280,181 @@ adamw32_kernel(const Args a, float *__restrict__ m, float *__restrict__ v) {
 // is zero, which would leave m / eps.  A gradient that is not finite makes
 // its block's scales, and so its states, not finite.
 
-constexpr unsigned ONE = 0x3F800000u;
-
 template <int BIAS, int SHIFT>
 SOD_DEVINL float grid(unsigned c) {
     return c ? __uint_as_float((c + BIAS) << SHIFT) : 0.f;
 }
 
-// x >= 0; at most the code of 1, below 1 for what is under the smallest code
-template <int BIAS, int SHIFT>
-SOD_DEVINL int code(float x, float inv, unsigned noise16) {
-    unsigned u = min(__float_as_uint(x * inv), ONE);
-    return (int)((u + (noise16 << (SHIFT - 16))) >> SHIFT) - BIAS;
+// The values of all codes, in LDS: a lookup where shifting, adding and the
+// exception for 0 take five operations and the sign two more.
+struct Tables { float m[256], r[256]; };
+
+// sqrt(v) correctly rounded, v a float32 under 2^63: the product with 1/sqrt
+// and one step of Heron's iteration, its residual exact, in place of sqrtf's
+// look at both neighbours.  The factors of 2^64 and 2^-32 keep the residual
+// of the smallest v a normal number; checked for every v.
+SOD_DEVINL float root(float v) {
+    float u = v * 0x1p64f;
+    float y = __builtin_amdgcn_rsqf(fmaxf(u, 0x1p-90f));    // 0 gives 0
+    float q = u * y;
+    float e = __builtin_fmaf(-q, q, u);
+    return __builtin_fmaf(e, 0.5f * y, q) * 0x1p-32f;
 }
 
 // the largest bits over 32 lanes (floats >= 0 compare like their bits, and
-// NaN above all)
+// NaN above all); the exchanges stay in the vector registers
 SOD_DEVINL unsigned max32lanes(unsigned v) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-        v = max(v, (unsigned)__shfl_xor((int)v, off, 64));
-    return v;
+#define SOD_MAX_DPP(ctrl)                                                     \
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF,    \
+                                                     0xF, true))
+    SOD_MAX_DPP(0xB1);      // lanes 1 apart (quad permutation 1 0 3 2)
+    SOD_MAX_DPP(0x4E);      // 2 apart (2 3 0 1)
+    SOD_MAX_DPP(0x141);     // the other 4 of 8 (mirrored)
+    SOD_MAX_DPP(0x140);     // the other 8 of 16 (mirrored)
+#undef SOD_MAX_DPP
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((unsigned)r[0], (unsigned)r[1]);
 }
 
-template <typename P, typename G>
-SOD_DEVINL void chunk8(const Args &a, const Info &I, const Row &R, long off,
-                       unsigned char *cm_, unsigned char *cr_, float2 *sc_,
-                       float gs, const Scalars &s) {
-    P *p = reinterpret_cast<P *>(R.param);
-    const G *g_ = reinterpret_cast<const G *>(R.grad);
-    long end = min(off + (long)CHUNK, I.numel);
-    // 32 lanes have a block; lanes past the end take part with zeros
-    for (long base = off; base < end; base += 2048) {
-        long i = base + threadIdx.x * 8;
-        long n = I.numel - i;
-        bool mine = (i & ~(long)(BLOCK - 1)) < I.numel;  // block has elements
-        f32x4 g[2], w[2];
-        uint2 cm = {0, 0}, cr = {0, 0};
-        float2 sc = make_float2(0.f, 0.f);
-        long blk = (I.state + i) / BLOCK;
+SOD_DEVINL unsigned sub_sat(unsigned a, unsigned b) {
+    return __builtin_elementwise_sub_sat(a, b);
+}
+
+// the top bytes of four words
+SOD_DEVINL unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0703u);
+    unsigned hi = __builtin_amdgcn_perm(d, c, 0x0c0c0703u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
+template <typename P, typename G, bool FULL>
+SOD_DEVINL void step8(const Args &a, const Info &I, const Row &R, int tensor,
+                      long off, unsigned char *cm_, unsigned char *cr_,
+                      float2 *sc_, Tables &tab, float gs) {
+    // 32 lanes have a block; lanes past the tensor's end take part with zeros.
+    // A lane has 4 elements of either half: every load and store of the 32 is
+    // one stretch, without which the non-temporal ones write lines in parts.
+    const long first = off + (threadIdx.x >> 5) * BLOCK;    // of the block
+    const bool mine = FULL || first < I.numel;
+    const long i = first + (threadIdx.x & 31) * 4, n = I.numel - i;
+    const long blk = (I.state + first) / BLOCK;
+    SOD_GLOBAL P *p = global_ptr<P>(R.param) + i;
+    const SOD_GLOBAL G *g_ = global_ptr<G>(R.grad) + i;
+    unsigned *cmp = reinterpret_cast<unsigned *>(cm_ + I.state + i);
+    unsigned *crp = reinterpret_cast<unsigned *>(cr_ + I.state + i);
+    f32x4 *wp = reinterpret_cast<f32x4 *>(a.master + I.master + i);
+    typename Vec4<G>::type g[2];
+    f32x4 w[2] = {};
+    unsigned cm[2] = {}, cr[2] = {};
+    float2 sc = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        g[h] = load4<G, FULL>(g_ + 128 * h, n - 128 * h);
+    if (mine) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            g[h] = load4(g_ + i + 4 * h, n - 4 * h);
-            if constexpr (sizeof(P) == 4) w[h] = load4(p + i + 4 * h, n - 4 * h);
-            else if (mine)
-                w[h] = *reinterpret_cast<f32x4 *>(a.master + I.master + i + 4 * h);
-            else w[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            cm[h] = __builtin_nontemporal_load(cmp + 32 * h);
+            cr[h] = __builtin_nontemporal_load(crp + 32 * h);
         }
-        if (mine) {
-            cm = *reinterpret_cast<uint2 *>(cm_ + I.state + i);
-            cr = *reinterpret_cast<uint2 *>(cr_ + I.state + i);
-            sc = sc_[blk];
-        }
-        float m[8], r[8];
-        unsigned mm = 0, mr = 0;
+        sc = sc_[blk];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (sizeof(P) == 4)
+            w[h] = load4<P, FULL>(p + 128 * h, n - 128 * h);
+        else if (mine) w[h] = __builtin_nontemporal_load(wp + 32 * h);
+    }
+    {
+        unsigned c = threadIdx.x;
+        float x = grid<889, 20>(c & 127u);
+        tab.m[c] = c & 128u ? -x : x;
+        tab.r[c] = grid<1777, 19>(c);
+    }
+    const Scalars s = step_scalars(a, I.wd, tensor, off);
+
+    f32x4 gf[2] = {to_f32(g[0], G()), to_f32(g[1], G())};
+    float m[8], r[8], v[8];
+    float mm = 0.f;
+    unsigned mr = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        unsigned c = (cm[e >> 2] >> (8 * (e & 3))) & 255u;
+        unsigned d = (cr[e >> 2] >> (8 * (e & 3))) & 255u;
+        float m0 = tab.m[c] * sc.x, r0 = tab.r[d] * sc.y;
+        float x = gf[e >> 2][e & 3] * gs;
+        m[e] = a.fb1 * m0 + a.fc1 * x;
+        v[e] = a.fb2 * (r0 * r0) + (a.fc2 * x) * x;
+        r[e] = root(v[e]);
+        mm = fmaxf(mm, fabsf(m[e]));
+        mr = max(mr, __float_as_uint(r[e]));
+    }
+    mr = max32lanes(mr);
+    if (__any(mr >= 0x4F000000u)) {     // r of 2^31 or more, or not finite
+        mr = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            unsigned c = ((e < 4 ? cm.x : cm.y) >> (8 * (e & 3))) & 255u;
-            unsigned d = ((e < 4 ? cr.x : cr.y) >> (8 * (e & 3))) & 255u;
-            float m0 = grid<889, 20>(c & 127u) * sc.x;
-            if (c & 128u) m0 = -m0;
-            float r0 = grid<1777, 19>(d) * sc.y;
-            float x = g[e >> 2][e & 3] * gs;
-            m[e] = a.fb1 * m0 + a.fc1 * x;
-            float v = a.fb2 * (r0 * r0) + (a.fc2 * x) * x;
-            r[e] = sqrtf(v);
-            w[e >> 2][e & 3] = moved(w[e >> 2][e & 3], m[e], r[e], a.eps, s);
-            mm = max(mm, __float_as_uint(fabsf(m[e])));
+            r[e] = sqrtf(v[e]);
             mr = max(mr, __float_as_uint(fabsf(r[e])));
         }
-        mm = max32lanes(mm);
         mr = max32lanes(mr);
-        float sm = __uint_as_float(mm), sr = __uint_as_float(mr);
-        // NaN stays NaN: the comparison is false
-        float im = 1.f / (sm < 0x1p-100f ? 0x1p-100f : sm);
-        float ir = 1.f / (sr < 0x1p-100f ? 0x1p-100f : sr);
-        cm = {0, 0};
-        cr = {0, 0};
+    }
+    float sr = __uint_as_float(mr);
+    float sm = __uint_as_float(max32lanes(__float_as_uint(mm)));
+    if (!(sr < INFINITY)) sm = sr;      // a NaN passes fmaxf by
+    float im = 1.f / fmaxf(sm, 0x1p-100f), ir = 1.f / fmaxf(sr, 0x1p-100f);
+    unsigned bm[8], br[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            unsigned h = mix32((unsigned)(i + e) + s.key);
-            int c = code<889, 20>(fabsf(m[e]), im, h >> 16);
-            if (c < 0) c = 0;
-            if (m[e] < 0.f && c > 0) c |= 128;
-            int d = code<1777, 19>(r[e], ir, h & 0xFFFFu);
-            if (d < 1) d = 1;
-            if (!(r[e] > 0.f)) d = 0;
-            (e < 4 ? cm.x : cm.y) |= (unsigned)c << (8 * (e & 3));
-            (e < 4 ? cr.x : cr.y) |= (unsigned)d << (8 * (e & 3));
-        }
-        if (mine) {
-            *reinterpret_cast<uint2 *>(cm_ + I.state + i) = cm;
-            *reinterpret_cast<uint2 *>(cr_ + I.state + i) = cr;
-            if ((threadIdx.x & 31) == 0) sc_[blk] = make_float2(sm, sr);
-        }
+    for (int e = 0; e < 8; ++e) {
+        unsigned h = mix32((unsigned)i + (e >> 2) * 128 + (e & 3) + s.key);
+        // 1 * scale ends up at 127 << 20 and 255 << 19; the code is what is
+        // left above the random bits, moved into the top byte
+        unsigned u = sub_sat(__float_as_uint(fabsf(m[e]) * im), 889u << 20);
+        u = ((h >> 16) << 4) + u;
+        bm[e] = ((u << 4) & 0x7FFFFFFFu) | (__float_as_uint(m[e]) & 0x80000000u);
+        unsigned d = sub_sat(__float_as_uint(r[e] * ir), 1777u << 19);
+        d = ((h & 0xFFFFu) << 3) + d;
+        // the middle one of the code, 1 and r's bits: at least 1, unless r is 0
+        // (and d noise below 1); the bits of any other r are above every code
+        d = max(min(d, 1u << 19), min(max(d, 1u << 19), __float_as_uint(r[e])));
+        br[e] = d << 5;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        w[e >> 2][e & 3] = moved(w[e >> 2][e & 3], m[e], r[e], a.eps, s);
+    if (mine) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if constexpr (sizeof(P) != 4)
-                if (mine)
-                    *reinterpret_cast<f32x4 *>(a.master + I.master + i + 4 * h) = w[h];
-            store4(p + i + 4 * h, n - 4 * h, w[h]);
+            unsigned *x = bm + 4 * h, *y = br + 4 * h;
+            __builtin_nontemporal_store(top_bytes(x[0], x[1], x[2], x[3]), cmp + 32 * h);
+            __builtin_nontemporal_store(top_bytes(y[0], y[1], y[2], y[3]), crp + 32 * h);
         }
+        if ((threadIdx.x & 31) == 0) sc_[blk] = make_float2(sm, sr);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (sizeof(P) != 4)
+            if (mine) __builtin_nontemporal_store(w[h], wp + 32 * h);
+        store4<P, FULL>(p + 128 * h, n - 128 * h, w[h]);
     }
 }
 
 __global__ void __launch_bounds__(256)
 adamw8_kernel(const Args a, unsigned char *__restrict__ cm,
               unsigned char *__restrict__ cr, float2 *__restrict__ sc) {
+    __shared__ Tables tab;
     float gs;
     int2 c = a.chunks[blockIdx.x];
     Info I = a.info[c.x];
     Row R = a.rows[c.x];
     if (R.grad == nullptr || !scaled(a, gs)) return;
-    long off = (long)c.y * CHUNK;
-    Scalars s = step_scalars(a, I.wd, c.x, off);
     by_types(I.dtype, R.grad_dtype, [&](auto p, auto g) {
-        chunk8<typename decltype(p)::type, typename decltype(g)::type>(
-            a, I, R, off, cm, cr, sc, gs, s);
+        using P = typename decltype(p)::type;
+        using G = typename decltype(g)::type;
+        long off = (long)c.y * CHUNK8;
+        if (off + CHUNK8 <= I.numel)
+            step8<P, G, true>(a, I, R, c.x, off, cm, cr, sc, tab, gs);
+        else
+            step8<P, G, false>(a, I, R, c.x, off, cm, cr, sc, tab, gs);
     });
 }
 
@@ -436,6 +521,7 @@ class AdamWPlan {
         std::vector<int64_t> info;          // Info's bytes
         std::vector<int> chunks;
         long places = 0, mplaces = 0;
+        const long chunk = moments_.size() == 2 ? CHUNK32 : CHUNK8;
         for (size_t i = 0; i < T; ++i) {
             auto &p = params_[i];
             TORCH_CHECK(p.device() == dev_,
@@ -456,9 +542,9 @@ class AdamWPlan {
                 mplaces += pad;
             }
             first_.push_back((int64_t)chunks.size() / 2);
-            for (long off = 0; off < I.numel; off += CHUNK) {
+            for (long off = 0; off < I.numel; off += chunk) {
                 chunks.push_back((int)i);
-                chunks.push_back((int)(off / CHUNK));
+                chunks.push_back((int)(off / chunk));
             }
             int64_t raw[sizeof(Info) / 8];
             memcpy(raw, &I, sizeof(I));

@@ -340,7 +340,7 @@ def adamw8_encode(m, r, noise):
     noise = noise.view(-1, ADAMW_BLOCK)
     sm, sr = m.abs().amax(1, keepdim=True), r.amax(1, keepdim=True)
     cm = codes(m.abs(), sm, (noise >> 16).to(torch.int32), 889, 20).clamp(min=0)
-    cm = torch.where((m < 0) & (cm > 0), cm + 128, cm)
+    cm = torch.where(torch.signbit(m), cm + 128, cm)
     cr = codes(r, sr, (noise & 0xFFFF).to(torch.int32), 1777, 19).clamp(min=1)
     cr = torch.where(r > 0, cr, torch.zeros_like(cr))
     return (cm.to(torch.uint8).view(-1), cr.to(torch.uint8).view(-1),
