@@ -601,6 +601,7 @@ class AdamWPlan {
               double gscale, torch::Tensor scale, int64_t seed) {
         using namespace sodkit::aw;
         if (n_chunks_ == 0) return;
+        at::NoGradGuard no_grad;
         c10::DeviceGuard guard(dev_);
         auto stream = at::hip::getCurrentHIPStream();
         Args a;
@@ -658,7 +659,7 @@ class AdamWPlan {
                         "adamw: parameter ", i, " has changed its size, type, "
                         "device or layout since the optimizer was made");
             const auto &src = grads_[i];
-            torch::Tensor g = src.defined() && src.numel() ? src : p.grad();
+            const auto &g = src.defined() && src.numel() ? src : p.grad();
             now[i] = {p.data_ptr(), nullptr, 0};
             if (!g.defined()) continue;
             TORCH_CHECK(g.layout() == torch::kStrided && g.device() == dev_ &&
@@ -668,11 +669,11 @@ class AdamWPlan {
             now[i].grad_dtype = type_code(g, "gradient");
             if (!same_order(g, p)) {
                 // elements are paired by their place in storage
-                g = torch::empty_strided(p.sizes(), p.strides(), g.options())
-                        .copy_(g);
-                copies.push_back(g);
-            }
-            now[i].grad = g.data_ptr();
+                copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
+                                                      g.options()).copy_(g));
+                now[i].grad = copies.back().data_ptr();
+            } else
+                now[i].grad = g.data_ptr();
         }
         if (rows_.defined() && now == host_) {
             if (capturing()) kept_ = true;

@@ -119,9 +119,8 @@ void sgd_fused(torch::Tensor ptrs, torch::Tensor numels, torch::Tensor wds,
                double gscale, bool nesterov, torch::Tensor scale,
                torch::Tensor lr_t);
 
-std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads,
-                                     double prescale, double max_norm,
-                                     torch::Tensor loss_scale,
+std::vector<torch::Tensor> grad_norm(pybind11::list grads, double prescale,
+                                     double max_norm, torch::Tensor loss_scale,
                                      torch::Tensor good, torch::Tensor skips,
                                      double growth);
 // AdamWPlan, adamw8_decode (csrc/adamw.hip)

@@ -27,10 +27,11 @@ from typing import Iterable
 
 import torch
 
-from . import reference
+from . import conv, reference
 from ._backend import ext
 
 _BLOCK = 256  # elements of an 8-bit block (must match csrc/adamw.hip)
+_NONE = torch.Tensor()
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -124,12 +125,14 @@ class SodAdamW:
         self.state: dict[torch.nn.Parameter, dict] = {}
         self._offsets, self._master_offsets, self._steps = [], [], []
         at = mat = 0
+        masters, rounded = [], []
         for p in self._params:
             n, pad = p.numel(), _padded(p.numel())
             st = {}
             if p.dtype != torch.float32:
                 st["master"] = self._master.as_strided(p.shape, p.stride(), mat)
-                st["master"].copy_(p.detach())
+                masters.append(st["master"])
+                rounded.append(p.detach())
             if self.state_bits == 32:
                 for k, f in zip(("exp_avg", "exp_avg_sq"), self._moments):
                     st[k] = f.as_strided(p.shape, p.stride(), at)
@@ -143,6 +146,8 @@ class SodAdamW:
             self._steps.append(0)           # CPU path; the GPU has its own
             at += pad
             mat += pad if p.dtype != torch.float32 else 0
+        if masters:
+            torch._foreach_copy_(masters, rounded)
 
     # -- flat states ---------------------------------------------------------
     @property
@@ -198,8 +203,8 @@ class SodAdamW:
     def grad_src(self, views) -> None:
         self._grad_src = views
         if self._plan is not None:
-            none = torch.Tensor()
-            self._plan.set_grads([(views or {}).get(p, none) for p in self._params])
+            views = views or {}
+            self._plan.set_grads([views.get(p, _NONE) for p in self._params])
 
     def _make_plan(self) -> None:
         """The kernel's tables, on the GPU: made ahead of the first step, which
@@ -213,7 +218,6 @@ class SodAdamW:
             self._plan.set_steps(self._steps)
             self.grad_src = self._grad_src
 
-    @torch.no_grad()
     def step(self, lr, grad_scale: float = 1.0,
              scale_t: "torch.Tensor | None" = None) -> None:
         """``lr`` and ``scale_t`` as in ``SodSGD.step``: ``scale_t``, a float32
@@ -225,18 +229,23 @@ class SodAdamW:
         if self._params[0].device != self._master.device:
             raise RuntimeError("the parameters have moved to another device "
                                "since the optimizer was made")
-        if self._plan is not None:
-            none = torch.Tensor()
-            on_gpu = isinstance(lr, torch.Tensor) and lr.is_cuda
-            self._plan.step(0.0 if on_gpu else float(lr),
-                            lr if on_gpu else none, *self.betas, self.eps,
-                            float(grad_scale),
-                            none if scale_t is None else scale_t, self.seed)
-            # weights just changed: re-transpose every cached dgrad w_t in
-            # one launch (sodkit/ops/conv.py _WtCache)
-            from . import conv as _conv
-            _conv._WtCache.refresh()
+        if self._plan is None:
+            self._step_cpu(lr, grad_scale, scale_t)
             return
+        lr_t = _NONE
+        if isinstance(lr, torch.Tensor):
+            if lr.is_cuda:
+                lr, lr_t = 0.0, lr
+            else:
+                lr = float(lr)
+        self._plan.step(lr, lr_t, *self.betas, self.eps, grad_scale,
+                        _NONE if scale_t is None else scale_t, self.seed)
+        # weights just changed: re-transpose every cached dgrad w_t in
+        # one launch (sodkit/ops/conv.py _WtCache)
+        conv._WtCache.refresh()
+
+    @torch.no_grad()
+    def _step_cpu(self, lr, grad_scale, scale_t) -> None:
         gs = torch.tensor(float(grad_scale))
         if scale_t is not None:
             if float(scale_t) == 0.0:

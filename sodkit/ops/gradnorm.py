@@ -12,8 +12,9 @@ import torch
 from . import reference
 from ._backend import ext
 
+_NONE = torch.Tensor()
 
-@torch.no_grad()
+
 def grad_norm(grads: Sequence[torch.Tensor], prescale: float = 1.0,
               max_norm: float = 0.0,
               loss_scale: Optional[torch.Tensor] = None,
@@ -38,7 +39,8 @@ def grad_norm(grads: Sequence[torch.Tensor], prescale: float = 1.0,
     Gradients may be float32, bfloat16 and float16, mixed, with any strides,
     on one device.  The sum is held in 64 bits and a repeated call gives the
     same bits."""
-    grads = list(grads)
+    if not isinstance(grads, list):
+        grads = list(grads)
     if not grads:
         raise ValueError("grad_norm needs at least one gradient")
     if (good_steps is None) != (skips is None) or (
@@ -48,12 +50,11 @@ def grad_norm(grads: Sequence[torch.Tensor], prescale: float = 1.0,
     if growth_interval < 1:
         raise ValueError(f"growth_interval must be positive, got {growth_interval}")
     if grads[0].is_cuda:
-        none = torch.Tensor()
         norm, mult = ext().grad_norm(
-            grads, float(prescale), float(max_norm),
-            none if loss_scale is None else loss_scale,
-            none if good_steps is None else good_steps,
-            none if skips is None else skips, float(growth_interval))
+            grads, prescale, max_norm,
+            _NONE if loss_scale is None else loss_scale,
+            _NONE if good_steps is None else good_steps,
+            _NONE if skips is None else skips, growth_interval)
         return norm, mult
     return reference.grad_norm(grads, prescale, max_norm, loss_scale,
                                good_steps, skips, growth_interval)
