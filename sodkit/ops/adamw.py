@@ -67,9 +67,13 @@ class SodAdamW:
     parameters.  They may be written in place, not replaced.
 
     A parameter whose gradient is None is left alone, its step count too.  A
-    gradient that is not finite makes its block's moments not finite where they
-    are held in 8 bits; ``ops.grad_norm`` gives the multiplier that skips such
-    a step."""
+    gradient that is not finite, or whose square is not, makes its block's
+    moments not finite where they are held in 8 bits; ``ops.grad_norm`` gives
+    the multiplier that skips such a step.
+
+    A step may be captured into a graph; ``betas``, ``eps``, ``seed`` and host
+    values of ``lr`` and ``grad_scale`` are then the capture's, the states, step
+    counts, decay and device scalars what they are at each replay."""
 
     def __init__(self, param_groups, betas: "tuple[float, float]" = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -102,6 +106,10 @@ class SodAdamW:
             if not _dense(p):
                 raise ValueError("parameters must be dense and without "
                                  f"overlaps, got strides {p.stride()} of {tuple(p.shape)}")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for p in self._params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters overlap in memory")
         self._grad_src = None
         self._allocate()
         self._make_plan()
@@ -206,15 +214,17 @@ class SodAdamW:
             views = views or {}
             self._plan.set_grads([views.get(p, _NONE) for p in self._params])
 
+    def _decay(self) -> "list[float]":
+        return [g["weight_decay"] for g in self.groups for _ in g["params"]]
+
     def _make_plan(self) -> None:
         """The kernel's tables, on the GPU: made ahead of the first step, which
         may be a captured one."""
         self._plan = None
         if self._params and self._params[0].is_cuda:
-            wd = [g["weight_decay"] for g in self.groups for _ in g["params"]]
-            self._plan = ext().AdamWPlan(self._params, wd, self._offsets,
-                                         self._master_offsets, self._master,
-                                         self._moments)
+            self._plan = ext().AdamWPlan(self._params, self._decay(),
+                                         self._offsets, self._master_offsets,
+                                         self._master, self._moments)
             self._plan.set_steps(self._steps)
             self.grad_src = self._grad_src
 
@@ -327,7 +337,9 @@ class SodAdamW:
         self._steps = [int(st["step"]) for st in saved]
         for g, wd in zip(self.groups, sd["group_wd"]):
             g["weight_decay"] = wd
-        self._make_plan()
+        if self._plan is not None:      # in place: captured steps live on
+            self._plan.set_decay(self._decay())
+            self._plan.set_steps(self._steps)
 
     def params(self) -> Iterable[torch.nn.Parameter]:
         for g in self.groups:

@@ -246,6 +246,9 @@ def test_refusals():
         SodAdamW([{"params": [torch.nn.Parameter(torch.ones(8)[::2])]}])
     with pytest.raises(ValueError, match="dense"):
         SodAdamW([{"params": [torch.nn.Parameter(torch.ones(1).expand(4))]}])
+    flat = torch.ones(6)
+    with pytest.raises(ValueError, match="overlap"):
+        SodAdamW([{"params": [torch.nn.Parameter(flat[:4]), torch.nn.Parameter(flat[3:])]}])
     opt = SodAdamW(ok)
     with pytest.raises(AttributeError):
         opt.code_m

@@ -265,6 +265,54 @@ def test_resume_on_gpu():
         assert other.state_dict()["param_state"][1]["step"] == 2
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_under_a_captured_step(bits):
+    """A state loaded after the capture is what the replays go on from."""
+    cpu, gpu = pair([(5000,), (33,)], torch.bfloat16, bits)
+    (ps, src, opt), (qs, gsrc, gopt) = cpu, gpu
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gopt.step(1e-2)
+    for o in (opt, gopt):
+        saved = SodAdamW([{"params": list(g["params"]), "weight_decay": 0.3}
+                          for g in o.groups], state_bits=bits, seed=11)
+        saved.grad_src = o.grad_src
+        before = [p.detach().clone() for p in saved.params()]
+        saved.step(1e-3)
+        saved.step(1e-3)
+        sd = {k: v for k, v in saved.state_dict().items()}
+        for p, b in zip(saved.params(), before):
+            p.data.copy_(b)
+        o.load_state_dict(sd)
+        del saved
+    for i in range(3):
+        graph.replay()
+        opt.step(1e-2)
+        same(cpu, gpu)
+    assert opt.state_dict()["group_wd"] == [0.3, 0.3]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_wide_range(bits):
+    """Gradients from denormal squares to roots past 2^31, zeros among them."""
+    gen = torch.Generator().manual_seed(2)
+    n = 40000
+    g = torch.randn(n, generator=gen) * 10.0 ** (torch.rand(n, generator=gen) * 46 - 28)
+    g[::7] = 0.0
+    g[:2048] *= 1e-22
+    sides = []
+    for d in ("cpu", "cuda"):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, n).to(d))
+        p.grad = g.to(d, copy=True)
+        opt = SodAdamW([{"params": [p]}], state_bits=bits, seed=1)
+        for _ in range(2):
+            opt.step(1e-2)
+            p.grad *= 0.3
+        sides.append(([p], None, opt))
+    same(*sides)
+
+
 def test_past_32_bits():
     """An element's place passes 2^32: the last elements move as the CPU's do."""
     if torch.cuda.mem_get_info()[0] < 80 << 30:
