@@ -10,6 +10,11 @@
 // sum of 1e9 terms keeps its low digits.  Every block writes one partial sum
 // and a second kernel adds them in a fixed order (no atomics), so a repeated
 // call gives the same bits.
+//
+// Bound by memory where there is much (1.56G bfloat16: 455 us, 6.9 TB/s), by
+// the two dependent launches where there is little: 24.5M bfloat16 take 14 us,
+// 11 and 3 of them the launches', where their bytes take 9.  A next chunk
+// loaded while one is added up changes neither.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -25,7 +30,8 @@ constexpr int SEGS = 160;       // tensors of one launch: 21 bytes each, and a
 //                                 kernel's arguments hold 4096
 constexpr int CHUNK = 8192;     // elements that a block reads at a time
 constexpr int MAX_BLOCKS = 8192;
-constexpr long SMALL = 16384;   // elements that one workgroup sums by itself
+constexpr long SMALL = 16384;   // elements that one workgroup sums by itself:
+//                                 111 vectors 6.9 us, in two launches 10.6
 
 // The tensors travel as kernel arguments: nothing to allocate, to copy or to
 // keep, and a captured graph has its own.
@@ -55,7 +61,7 @@ SOD_DEVINL float elem(const typename Vec<T>::type &v, int i, T) {
 }
 
 template <typename T>
-SOD_DEVINL double chunk_sum(const T *p, long n) {
+SOD_DEVINL double chunk_sum(const T *p, int n) {
     using V = typename Vec<T>::type;
     constexpr int W = 16 / sizeof(T);
     double a[4] = {0., 0., 0., 0.};
@@ -76,7 +82,7 @@ SOD_DEVINL double chunk_sum(const T *p, long n) {
                 }
         }
     } else {
-        for (long i = threadIdx.x; i < n; i += 256) {
+        for (int i = threadIdx.x; i < n; i += 256) {
             double x = (double)ElemTraits<T>::to_f32(p[i]);
             a[0] = fma(x, x, a[0]);
         }
@@ -104,8 +110,11 @@ norm_partial_kernel(const Segs segs, double *__restrict__ partial) {
             if (segs.first[mid] <= c) lo = mid; else hi = mid - 1;
         }
         long off = (long)(c - segs.first[lo]) * CHUNK;
-        long n = segs.numel[lo] - off;
-        if (n > CHUNK) n = CHUNK;
+        long left = segs.numel[lo] - off;
+        // The comparison in 32 bits (CHUNK is a power of two): of a uniform
+        // 64-bit one and its selections the compiler (ROCm 7.2) has put an
+        // addition in between, whose carry the selections took for its result.
+        int n = (int)(left / CHUNK) != 0 ? CHUNK : (int)left;
         const void *p = segs.ptr[lo];
         int d = segs.dtype[lo];
         if (d == 0)

@@ -395,6 +395,21 @@ def test_grad_norm(dtype, sizes):
     assert differ(norm, again[0]) == 0 and differ(mult, again[1]) == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [8192 * 2048 + 300, 8192 * 4096 + 1, 8192 * 2048 * 3 + 4097,
+                               8192 * 33000 + 300])
+def test_grad_norm_ends(dtype, n):
+    """Every piece counts: alone, the first elements and the last, as the first,
+    second and later piece of a workgroup."""
+    x = torch.zeros(n, dtype=dtype, device="cuda")
+    for part in (x[:300], x[-300:], x[-8193:-8192], x[n // 2:n // 2 + 1]):
+        part.fill_(2.0)
+        norm = grad_norm([x])[0].item()
+        want = 2.0 * math.sqrt(part.numel())
+        assert abs(norm - want) <= 2.0 ** -23 * want
+        part.zero_()
+
+
 def test_grad_norm_views_and_range():
     x = torch.randn(40, 30, device="cuda")
     mixed = [x.t(), x[::2, ::3], x[:1].expand(5, 30), x.bfloat16(), x.half()]
