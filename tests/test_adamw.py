@@ -5,11 +5,14 @@ import math
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from adamw_oracle import check, decode64, level, param_bound, step64
 from sodkit.config import make_config
 from sodkit.engine import Solver
 from sodkit.ops import SodAdamW, SodSGD, grad_norm, reference
+from sodkit.parallel import GradReducer
 
 HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, wd=0.1)
 
@@ -346,6 +349,68 @@ def test_grad_norm_refusals():
                   skips=torch.tensor(0.0))
     with pytest.raises(ValueError):
         grad_norm([torch.ones(3)], growth_interval=0)
+
+
+# ------------------------------------------------------------------ ranks
+
+def _net():
+    torch.manual_seed(7)
+    return torch.nn.Sequential(torch.nn.Linear(8, 50), torch.nn.ReLU(),
+                               torch.nn.Linear(50, 4))
+
+
+def _grads(m, rank, i):
+    """The gradients of a rank's data in step i."""
+    x = torch.full((2, 8), 0.1 * (rank + 1) * (i + 1)) + torch.arange(8) * 0.01
+    return torch.autograd.grad(m(x).square().sum(), list(m.parameters()))
+
+
+def _ranks_worker(rank, store, bits, q):
+    torch.set_num_threads(2)
+    dist.init_process_group("gloo", rank=rank, world_size=2,
+                            init_method=f"file://{store}")
+    m = _net()
+    red = GradReducer(m, bucket_mb=1)
+    opt = SodAdamW([{"params": list(m.parameters())}], state_bits=bits, seed=3)
+    opt.grad_src = red.grad_views
+    for i in range(3):
+        red.zero_grad()
+        x = torch.full((2, 8), 0.1 * (rank + 1) * (i + 1)) + torch.arange(8) * 0.01
+        m(x).square().sum().backward()
+        red.finalize()
+        _, mult = grad_norm([b.flat for b in red.buckets],
+                            prescale=red.grad_scale, max_norm=0.1)
+        opt.step(1e-2, red.grad_scale, scale_t=mult)
+    q.put((rank, [p.detach().clone() for p in m.parameters()]))
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_ranks_agree(bits, tmp_path):
+    """Two ranks end with the same bits, those of one process that adds up both
+    ranks' gradients."""
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_ranks_worker, args=(r, str(tmp_path / "s"), bits, q))
+             for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in range(2))
+    for p in procs:
+        p.join(60)
+    m = _net()
+    opt = SodAdamW([{"params": list(m.parameters())}], state_bits=bits, seed=3)
+    for i in range(3):
+        for p, a, b in zip(m.parameters(), _grads(m, 0, i), _grads(m, 1, i)):
+            p.grad = a + b
+        # the buckets' order: from the last parameter
+        _, mult = grad_norm([p.grad for p in reversed(list(m.parameters()))],
+                            prescale=0.5, max_norm=0.1)
+        opt.step(1e-2, 0.5, scale_t=mult)
+    for a, b, p in zip(got[0], got[1], m.parameters()):
+        assert torch.equal(a, b)
+        # (the norm's sum is grouped otherwise, in 64 bits: its float32 is the same)
+        assert torch.equal(a, p)
 
 
 # ------------------------------------------------------------------ the solver
