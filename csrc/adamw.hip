@@ -549,8 +549,9 @@ class AdamWPlan {
             I.master = master[i];
             I.wd = wd[i];
             I.dtype = type_code(p, "parameter");
-            dtypes_.push_back((int)I.dtype);
-            numels_.push_back(I.numel);
+            layouts_.push_back({p.scalar_type(), {}});
+            if (!p.is_contiguous())
+                layouts_.back().strides = p.strides().vec();
             long pad = (I.numel + BLOCK - 1) / BLOCK * BLOCK;
             TORCH_CHECK(I.state % BLOCK == 0 && I.state == places);
             places += pad;
@@ -606,7 +607,7 @@ class AdamWPlan {
         auto s = steps_.cpu();
         std::vector<int64_t> out;
         for (size_t i = 0; i < params_.size(); ++i)
-            out.push_back(numels_[i] ? s.data_ptr<int>()[first_[i]] : 0);
+            out.push_back(infos_[i].numel ? s.data_ptr<int>()[first_[i]] : 0);
         return out;
     }
 
@@ -679,12 +680,15 @@ class AdamWPlan {
                         std::vector<torch::Tensor> &copies) {
         using namespace sodkit::aw;
         size_t T = params_.size();
-        std::vector<Row> now(T);
+        now_.resize(T);
+        auto &now = now_;
         for (size_t i = 0; i < T; ++i) {
-            auto &p = params_[i];
-            TORCH_CHECK(p.numel() == numels_[i] && p.device() == dev_ &&
-                        type_code(p, "parameter") == dtypes_[i] &&
-                        p.is_non_overlapping_and_dense(),
+            const auto &p = params_[i];
+            const auto &l = layouts_[i];
+            TORCH_CHECK(p.numel() == infos_[i].numel && p.device() == dev_ &&
+                        p.scalar_type() == l.dtype &&
+                        (l.strides.empty() ? p.is_contiguous()
+                                           : p.strides() == l.strides),
                         "adamw: parameter ", i, " has changed its size, type, "
                         "device or layout since the optimizer was made");
             const auto &src = grads_[i];
@@ -696,7 +700,7 @@ class AdamWPlan {
                         "parameter ", i, " must be dense, of its size and on "
                         "its device");
             now[i].grad_dtype = type_code(g, "gradient");
-            if (!same_order(g, p)) {
+            if (!(l.strides.empty() && g.is_contiguous()) && !same_order(g, p)) {
                 // elements are paired by their place in storage
                 copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
                                                       g.options()).copy_(g));
@@ -753,11 +757,17 @@ class AdamWPlan {
     torch::Tensor masters_;
     std::vector<torch::Tensor> moments_;
     std::vector<sodkit::aw::Info> infos_;
-    std::vector<int> dtypes_;
-    std::vector<int64_t> numels_, first_;
+    // a parameter's order in storage, which is its states': contiguous (no
+    // strides kept) or these
+    struct Layout {
+        at::ScalarType dtype;
+        std::vector<int64_t> strides;
+    };
+    std::vector<Layout> layouts_;
+    std::vector<int64_t> first_;
     int64_t n_chunks_ = 0;
     torch::Tensor info_, chunks_, steps_, rows_;
-    std::vector<Row> host_;
+    std::vector<Row> host_, now_;           // rows_' content; this step's
     bool kept_ = false;                     // a captured graph reads rows_
     std::vector<torch::Tensor> graphs_;     // tables that graphs read
     c10::hip::HIPStream made_on_ = at::hip::getDefaultHIPStream();

@@ -110,6 +110,8 @@ class SodAdamW:
                        for p in self._params if p.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters overlap in memory")
+        self._shapes = [p.shape for p in self._params]
+        self._strides = [p.stride() for p in self._params]
         self._grad_src = None
         self._allocate()
         self._make_plan()
@@ -261,35 +263,36 @@ class SodAdamW:
             if float(scale_t) == 0.0:
                 return
             gs = gs * scale_t.to("cpu", torch.float32)
-        k = -1
-        for g in self.groups:
-            for p in g["params"]:
-                k += 1
-                grad = (self._grad_src or {}).get(p)
-                grad = p.grad if grad is None else grad
-                if grad is None:
-                    continue
-                if grad.layout != torch.strided or grad.shape != p.shape \
-                        or grad.dtype not in _DTYPES or grad.device != p.device:
-                    raise RuntimeError(
-                        f"the gradient of parameter {k} must be dense, of its "
-                        f"size, on its device and float32, bfloat16 or float16")
-                if p.numel() == 0:
-                    continue
-                grad = torch.empty_strided(p.shape, p.stride(), dtype=grad.dtype).copy_(grad)
-                self._steps[k] += 1
-                st = self.state[p]
-                w = _in_storage(st["master"] if "master" in st else p.data)
-                args = (float(lr), self._steps[k], self.betas, self.eps,
-                        g["weight_decay"], gs)
-                if self.state_bits == 32:
-                    reference.adamw_step(_in_storage(p.data), _in_storage(grad), w,
-                                         _in_storage(st["exp_avg"]),
-                                         _in_storage(st["exp_avg_sq"]), *args)
-                else:
-                    reference.adamw8_step(_in_storage(p.data), _in_storage(grad), w,
-                                          st["code_m"], st["code_r"], st["scales"],
-                                          *args, self.seed, k)
+        grads = []
+        for k, p in enumerate(self._params):
+            grad = (self._grad_src or {}).get(p)
+            grad = p.grad if grad is None else grad
+            grads.append(grad)
+            if p.shape != self._shapes[k] or p.stride() != self._strides[k]:
+                raise RuntimeError(f"parameter {k} has changed its size or "
+                                   f"layout since the optimizer was made")
+            if grad is not None and (
+                    grad.layout != torch.strided or grad.shape != p.shape
+                    or grad.dtype not in _DTYPES or grad.device != p.device):
+                raise RuntimeError(
+                    f"the gradient of parameter {k} must be dense, of its "
+                    f"size, on its device and float32, bfloat16 or float16")
+        for k, (p, grad, wd) in enumerate(zip(self._params, grads, self._decay())):
+            if grad is None or p.numel() == 0:
+                continue
+            grad = torch.empty_strided(p.shape, p.stride(), dtype=grad.dtype).copy_(grad)
+            self._steps[k] += 1
+            st = self.state[p]
+            w = _in_storage(st["master"] if "master" in st else p.data)
+            args = (float(lr), self._steps[k], self.betas, self.eps, wd, gs)
+            if self.state_bits == 32:
+                reference.adamw_step(_in_storage(p.data), _in_storage(grad), w,
+                                     _in_storage(st["exp_avg"]),
+                                     _in_storage(st["exp_avg_sq"]), *args)
+            else:
+                reference.adamw8_step(_in_storage(p.data), _in_storage(grad), w,
+                                      st["code_m"], st["code_r"], st["scales"],
+                                      *args, self.seed, k)
 
     def set_step(self, step: int) -> None:
         """Set every parameter's count of steps taken."""

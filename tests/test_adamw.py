@@ -271,6 +271,12 @@ def test_refusals():
     with pytest.raises(ValueError, match="fit"):
         SodAdamW([{"params": [torch.nn.Parameter(torch.ones(5))]}]).load_state_dict(
             opt.state_dict())
+    q = torch.nn.Parameter(torch.ones(2, 3, 4, 5))
+    opt = SodAdamW([{"params": [q]}])
+    q.data = q.data.contiguous(memory_format=torch.channels_last)
+    q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="layout"):
+        opt.step(0.1)
     assert SodAdamW([]).step(0.1) is None
 
 

@@ -365,6 +365,12 @@ def test_refusals():
     p.grad = torch.ones_like(p)
     with pytest.raises(RuntimeError, match="changed"):
         opt.step(0.1)
+    q = torch.nn.Parameter(torch.ones(2, 3, 4, 5, device="cuda"))
+    opt = SodAdamW([{"params": [q]}])
+    q.data = q.data.contiguous(memory_format=torch.channels_last)
+    q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="changed"):
+        opt.step(0.1)
     with pytest.raises(RuntimeError, match="loss_scale"):
         grad_norm([p.grad], loss_scale=torch.ones(()))
     with pytest.raises(RuntimeError, match="one device"):
