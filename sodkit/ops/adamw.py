@@ -227,6 +227,7 @@ class SodAdamW:
             self._plan = ext().AdamWPlan(self._params, self._decay(),
                                          self._offsets, self._master_offsets,
                                          self._master, self._moments)
+            self._plan_wd = [g["weight_decay"] for g in self.groups]
             self._plan.set_steps(self._steps)
             self.grad_src = self._grad_src
 
@@ -244,6 +245,10 @@ class SodAdamW:
         if self._plan is None:
             self._step_cpu(lr, grad_scale, scale_t)
             return
+        wd = [g["weight_decay"] for g in self.groups]
+        if wd != self._plan_wd:
+            self._plan.set_decay(self._decay())
+            self._plan_wd = wd
         lr_t = _NONE
         if isinstance(lr, torch.Tensor):
             if lr.is_cuda:
@@ -342,6 +347,7 @@ class SodAdamW:
             g["weight_decay"] = wd
         if self._plan is not None:      # in place: captured steps live on
             self._plan.set_decay(self._decay())
+            self._plan_wd = [g["weight_decay"] for g in self.groups]
             self._plan.set_steps(self._steps)
 
     def params(self) -> Iterable[torch.nn.Parameter]:

@@ -142,6 +142,15 @@ def test_layouts(bits):
         same(([ps[0]], None, opts[0]), ([ps[1]], None, opts[1]))
 
 
+def test_decay_that_changes():
+    cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
+    for wd in (0.1, 0.4):
+        for _, _, o in (cpu, gpu):
+            o.groups[0]["weight_decay"] = wd
+            o.step(1e-2)
+        same(cpu, gpu)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_skip(bits):
     _, (ps, src, opt) = pair([(5000,), (3,)], torch.bfloat16, bits)
