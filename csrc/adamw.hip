@@ -534,6 +534,7 @@ class AdamWPlan {
         TORCH_CHECK(!params_.empty() && params_[0].is_cuda());
         dev_ = params_[0].device();
         c10::DeviceGuard guard(dev_);
+        home_ = at::hip::getCurrentHIPStream();
         size_t T = params_.size();
         TORCH_CHECK(wd.size() == T && state.size() == T && master.size() == T);
         std::vector<int> chunks;
@@ -634,6 +635,13 @@ class AdamWPlan {
         a.scale = scalar(scale, "scale_t");
         std::vector<torch::Tensor> copies;      // until the launch is queued
         torch::Tensor rows = table(stream, copies);
+        if (stream != home_ && !capturing()) {
+            // whoever frees these waits for this stream too
+            c10::Stream here(c10::Stream::UNSAFE, dev_, stream.id());
+            for (auto *t : {&info_, &chunks_, &steps_, &masters_})
+                t->record_stream(here);
+            for (auto &t : moments_) t.record_stream(here);
+        }
         a.info = reinterpret_cast<const Info *>(info_.data_ptr());
         a.rows = reinterpret_cast<const Row *>(rows.data_ptr());
         a.chunks = reinterpret_cast<const int2 *>(chunks_.data_ptr());
@@ -770,7 +778,9 @@ class AdamWPlan {
     std::vector<Row> host_, now_;           // rows_' content; this step's
     bool kept_ = false;                     // a captured graph reads rows_
     std::vector<torch::Tensor> graphs_;     // tables that graphs read
-    c10::hip::HIPStream made_on_ = at::hip::getDefaultHIPStream();
+    // the streams that the states and that rows_ were allocated on
+    c10::hip::HIPStream home_ = at::hip::getDefaultHIPStream();
+    c10::hip::HIPStream made_on_ = home_;
 };
 
 // {m, v} of moments in 8 bits, bfloat16, in the states' places

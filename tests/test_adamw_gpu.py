@@ -259,6 +259,25 @@ def test_other_stream(bits):
     same(cpu, gpu)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_at_once(bits):
+    """Two optimizers and norms on two streams."""
+    cpu, gpu = pair([(300001,), (5,)], torch.bfloat16, bits)
+    _, other = pair([(300001,), (5,)], torch.bfloat16, bits)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(5):
+        for (ps, src, opt), st in zip((gpu, other), streams):
+            with torch.cuda.stream(st):
+                _, mult = grad_norm(list(src.values()), max_norm=1.0)
+                opt.step(1e-2, scale_t=mult)
+        _, mult = grad_norm(list(cpu[1].values()), max_norm=1.0)
+        cpu[2].step(1e-2, scale_t=mult)
+    torch.cuda.synchronize()
+    same(cpu, gpu)
+    same(cpu, other)
+
+
 def test_resume_on_gpu():
     for bits in (32, 8):
         _, (ps, src, opt) = pair([(5000,), (33,)], torch.bfloat16, bits)
