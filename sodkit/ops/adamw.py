@@ -55,6 +55,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _order(t: torch.Tensor) -> "tuple[int, ...]":
+    """The strides that matter."""
+    return tuple(st if sz > 1 else 0 for st, sz in zip(t.stride(), t.shape))
+
+
 class SodAdamW:
     """``param_groups``: dicts ``{"params": [...], "weight_decay": float}``, the
     decay defaulting to ``weight_decay``.  ``state_bits``: 32 or 8.
@@ -313,7 +318,7 @@ class SodAdamW:
         waits for the GPU)."""
         if self._plan is not None:
             self._steps = self._plan.get_steps()
-        flat = [{**self.state[p], "step": t}
+        flat = [{**self.state[p], "step": t, "order": _order(p)}
                 for p, t in zip(self._params, self._steps)]
         return {"kind": "adamw", "state_bits": self.state_bits,
                 "betas": self.betas, "eps": self.eps, "seed": self.seed,
@@ -333,10 +338,14 @@ class SodAdamW:
                              f"{len(self._params)} in {len(self.groups)}")
         for k, (p, st) in enumerate(zip(self._params, saved)):
             mine = self.state[p]
-            if set(st) - {"step"} != set(mine) or any(
+            if set(st) - {"step", "order"} != set(mine) or any(
                     st[n].shape != mine[n].shape for n in mine):
                 raise ValueError(f"checkpoint's state of parameter {k} does "
                                  f"not fit it")
+            # codes lie in the order of the parameter's storage
+            if self.state_bits == 8 and tuple(st["order"]) != _order(p):
+                raise ValueError(f"checkpoint's 8-bit state of parameter {k} is "
+                                 f"of another memory layout")
         self.betas, self.eps = tuple(sd["betas"]), sd["eps"]
         self.seed = sd["seed"]
         for p, st in zip(self._params, saved):

@@ -57,7 +57,7 @@ def same(a, b):
     for k, (x, y) in enumerate(zip(sa, sb)):
         assert x["step"] == y["step"]
         for n in x:
-            assert n == "step" or differ(x[n], y[n]) == 0, (k, n)
+            assert n in ("step", "order") or differ(x[n], y[n]) == 0, (k, n)
 
 
 @pytest.mark.parametrize("bits", [32, 8])
