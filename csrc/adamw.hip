@@ -17,7 +17,7 @@
 // It is bound by memory: 28 bytes an element, 16 with moments in 8 bits.  What
 // moves once a step passes the caches by (non-temporal), in whole lines:
 //   24.5M bfloat16 parameters   32 bits 107 us, 6.4 TB/s   8 bits 63 us, 6.2
-//   391M, float32 / bfloat16            1.88 ms, 5.8               1.02 ms, 6.2
+//   391M, float32 / bfloat16            1.84 ms, 6.0               1.02 ms, 6.2
 // where a large copy reaches 5.1 to 5.4 TB/s and a fill 6.9.
 
 #include <torch/extension.h>
@@ -98,13 +98,16 @@ template <> struct Vec4<__half> {
     typedef short type __attribute__((ext_vector_type(4), aligned(2)));
 };
 
-// A quad of a parameter or gradient.  FULL: all four lie in the tensor, and the
+// A quad of a parameter or gradient.  NT: past the caches.  FULL: all four lie in the tensor, and the
 // load is the only thing that happens (converted where it is used, so that
 // nothing waits for it between this and the next load).
-template <typename T, bool FULL>
+template <typename T, bool FULL, bool NT = false>
 SOD_DEVINL typename Vec4<T>::type load4(const SOD_GLOBAL T *p, long n) {
     using V = typename Vec4<T>::type;
-    if (FULL || n >= 4) return *(const SOD_GLOBAL V *)p;
+    if (FULL || n >= 4) {
+        const SOD_GLOBAL V *q = (const SOD_GLOBAL V *)p;
+        return NT ? __builtin_nontemporal_load(q) : *q;
+    }
     V r = {};
     for (int e = 0; e < 3; ++e)
         if (e < n) r[e] = ((const SOD_GLOBAL typename Vec4<T>::elem *)p)[e];
@@ -184,7 +187,8 @@ SOD_DEVINL float moved(float w, float m, float r, float eps, const Scalars &s) {
 // A thread has one quad, so that a CU has as many workgroups as it can and
 // their loads overlap: 116 us for 24.5M bfloat16 parameters, 120 with two or
 // four quads, 132 through the caches.  The parameter is written non-temporally
-// too (115 -> 107).  The scalars go first: with the loads in front of their
+// too (115 -> 107), and read so where it is its own master (391M float32
+// 1.89 -> 1.84 ms); gradients are not, the backward pass has just left them.  The scalars go first: with the loads in front of their
 // barrier tensors at odd addresses took 198 us and not 184, the others 1 % less.
 
 template <typename P, typename G, bool FULL>
@@ -203,7 +207,7 @@ SOD_DEVINL void step32(const Args &a, const Info &I, const Row &R, int tensor,
         gq = load4<G, FULL>(g_, n);
         m = __builtin_nontemporal_load(mp);
         v = __builtin_nontemporal_load(vp);
-        if constexpr (sizeof(P) == 4) w = load4<P, FULL>(p, n);
+        if constexpr (sizeof(P) == 4) w = load4<P, FULL, true>(p, n);
         else w = __builtin_nontemporal_load(wp);
     }
     if (!FULL && n <= 0) return;
@@ -294,7 +298,8 @@ adamw32_kernel(const Args a, float *__restrict__ m, float *__restrict__ v) {
 // where memory leaves time for 115: 99 us for 24.5M bfloat16 parameters.  With
 // the table, the root and the coding below it is 68, and 63 with the codes past
 // the caches (and the loads in front of the scalars' barrier; behind it 1 %
-// slower).  Quotients stay the compiler's, exact ones.
+// slower).  194M float32 parameters, their own masters, take 516 us read past
+// the caches, 564 through them.  Quotients stay the compiler's, exact ones.
 
 template <int BIAS, int SHIFT>
 SOD_DEVINL float grid(unsigned c) {
@@ -377,7 +382,7 @@ SOD_DEVINL void step8(const Args &a, const Info &I, const Row &R, int tensor,
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if constexpr (sizeof(P) == 4)
-            w[h] = load4<P, FULL>(p + 128 * h, n - 128 * h);
+            w[h] = load4<P, FULL, true>(p + 128 * h, n - 128 * h);
         else if (mine) w[h] = __builtin_nontemporal_load(wp + 32 * h);
     }
     {
