@@ -436,7 +436,7 @@ __global__ void bn_bwd_reduce_kernel(const T *__restrict__ dy,
 
 // ---- vectorized backward apply (C % 8 == 0) ----
 template <typename T, bool RELU, bool NEED_DRES, bool MASKED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 8)     // 64 registers: 8 waves a SIMD
 bn_bwd_apply_vec_kernel(const T *__restrict__ dy,
                                         const T *__restrict__ y,
                                         const T *__restrict__ x,
