@@ -339,6 +339,9 @@ def adamw8_encode(m, r, noise):
     m, r = m.view(-1, ADAMW_BLOCK), r.view(-1, ADAMW_BLOCK)
     noise = noise.view(-1, ADAMW_BLOCK)
     sm, sr = m.abs().amax(1, keepdim=True), r.amax(1, keepdim=True)
+    # a square past float32 leaves m finite beside an r that stops every step:
+    # neither moment of such a block is finite, as in the kernel
+    sm = torch.where(torch.isfinite(sr), sm, sr)
     cm = codes(m.abs(), sm, (noise >> 16).to(torch.int32), 889, 20).clamp(min=0)
     cm = torch.where(torch.signbit(m), cm + 128, cm)
     cr = codes(r, sr, (noise & 0xFFFF).to(torch.int32), 1777, 19).clamp(min=1)

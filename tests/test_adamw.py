@@ -202,6 +202,21 @@ def test_non_finite_gradient_is_loud():
     assert not torch.isfinite(opt2.scales[1]).any()
 
 
+@pytest.mark.parametrize("big", [2e21, 1e22, -3e38])
+def test_square_past_float32_is_loud(big):
+    """A finite gradient whose square is not (0.001 * g * g past 3.4e38) makes both
+    moments of its block not finite, and of no other."""
+    p, opt, gen = make(700, bits=8)
+    p.grad = torch.randn(700, generator=gen)
+    p.grad[300] = big
+    opt.step(0.1)
+    finite = torch.isfinite(opt.scales)
+    assert finite[0].all() and finite[2].all() and not finite[1].any()
+    for t in opt.moments():
+        assert not torch.isfinite(t[256:512]).any()
+        assert torch.isfinite(t[:256]).all() and torch.isfinite(t[512:]).all()
+
+
 def test_noise_past_32_bits():
     """Elements 2^32 apart have other noise, tensors and steps too."""
     a = reference.adamw8_noise(4, 1, 1, 0)

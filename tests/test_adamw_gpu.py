@@ -178,6 +178,24 @@ def test_non_finite_in_8_bits(bad):
         assert torch.isfinite(m[:256]).all() and torch.isfinite(m[512:]).all()
 
 
+@pytest.mark.parametrize("big", [2e21, -3e38])
+def test_square_past_float32_in_8_bits(big):
+    """The CPU and the GPU agree on the block that such a gradient takes away."""
+    cpu, gpu = pair([(1000,)], torch.float32, 8)
+    for ps, src, opt in (cpu, gpu):
+        src[ps[0]][300] = big
+        opt.step(1e-2)
+        opt.step(1e-2)
+        finite = torch.isfinite(opt.scales)
+        assert finite[[0, 2, 3]].all() and not finite[1].any()
+        for t in opt.moments():
+            assert not torch.isfinite(t[256:512]).any()
+            assert torch.isfinite(t[:256]).all() and torch.isfinite(t[512:]).all()
+    keep = torch.ones(1000, dtype=torch.bool)
+    keep[256:512] = False
+    assert differ(cpu[0][0][keep], gpu[0][0].cpu()[keep]) == 0
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_gradients_that_move(bits):
     """A new gradient each step, as autograd makes them, and weights that move."""
