@@ -148,8 +148,11 @@ SOD_DEVINL unsigned mix32(unsigned h) {
 
 // One wave works them out for its workgroup, another one from workgroup to
 // workgroup, as its SIMD has the time to give; its lanes 0 and 1 go through the
-// same float64 operations with b1 and b2: the power by squaring (a few units
-// of its last place, which rounding to float32 takes up), root and quotient.
+// same float64 operations with b1 and b2: the power by squaring, root and
+// quotient.  A squaring doubles the relative error that it gets, so the power's
+// grows with t, under t * 2^-53 (2^-33 after a million steps, where a float32
+// has 2^-24).  That can still decide a rounding to float32: the CPU's path
+// goes through the same products (reference._power).
 SOD_DEVINL Scalars step_scalars(const Args &a, double wd, int tensor, long off) {
     __shared__ Scalars sh;
     if ((threadIdx.x >> 6) == (blockIdx.x & 3)) {

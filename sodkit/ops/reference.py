@@ -272,10 +272,25 @@ def _root(v):
     return v.double().sqrt().float()
 
 
+def _power(b: float, step: int) -> float:
+    """b^step by squaring, each product rounded to float64 as in the kernel.
+    A squaring doubles the error that it gets, so the error grows with step:
+    under step * 2^-53, relative.  `**` is nearer, but not the same bits, and
+    1 - b^step takes the difference into the last bit of a float32 now and
+    then where b is near one."""
+    p = 1.0
+    while step:
+        if step & 1:
+            p *= b
+        b *= b
+        step >>= 1
+    return p
+
+
 def _adamw_weight(param, w, m, r, lr, step, betas, eps, weight_decay):
     b1, b2 = betas
-    rate = lr / (1 - b1 ** step)
-    den = r * (1 / math.sqrt(1 - b2 ** step)) + eps
+    rate = lr / (1 - _power(b1, step))
+    den = r * (1 / math.sqrt(1 - _power(b2, step))) + eps
     new = w * (1 - lr * weight_decay) - (m / den) * rate
     w.copy_(new)
     if param.dtype == torch.float16:      # saturates, as every kernel's cast

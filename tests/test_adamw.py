@@ -61,6 +61,37 @@ def test_matches_torch_adamw():
     assert ((p - q).abs() <= bound).all()
 
 
+LONG_RUNS = [((0.9, 0.999999), 1e-3, 12314), ((0.9, 0.999999), 1e-3, 155629),
+             ((0.99999, 0.999), 1e-4, 20739), ((0.999999, 0.999), 1e-3, 5943),
+             ((0.9, 0.999), 1e-3, 400000)]
+
+
+@pytest.mark.parametrize("betas, lr, t", LONG_RUNS)
+def test_late_steps_go_by_the_kernels_products(betas, lr, t):
+    """b^t comes from squarings, rounded one by one, whose error at these steps
+    decides a float32: the step is the one with the scalars that they give."""
+    def power(b, k):
+        out = 1.0
+        for bit in reversed(bin(k)[2:]):
+            out = out * b if bit == "1" else out
+            b = b * b
+        return out
+
+    g = torch.Generator().manual_seed(0)
+    p = torch.nn.Parameter(torch.zeros(4096))
+    opt = SodAdamW([{"params": [p], "weight_decay": 0.0}], betas=betas)
+    opt.exp_avg.copy_(torch.randn(4096, generator=g))
+    opt.exp_avg_sq.copy_(torch.rand(4096, generator=g))
+    opt.set_step(t - 1)
+    p.grad = torch.zeros(4096)
+    opt.step(lr)
+    rate = torch.tensor(lr / (1 - power(betas[0], t)), dtype=torch.float32)
+    rbc2 = torch.tensor(1 / math.sqrt(1 - power(betas[1], t)), dtype=torch.float32)
+    r = opt.exp_avg_sq.double().sqrt().float()
+    want = -(rate * (opt.exp_avg / (r * rbc2 + torch.tensor(1e-8))))
+    assert torch.equal(p.detach(), want)
+
+
 def test_groups_scale_and_skip():
     ps = [torch.nn.Parameter(torch.ones(5)) for _ in range(3)]
     opt = SodAdamW([{"params": ps[:1], "weight_decay": 0.5},

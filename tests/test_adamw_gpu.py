@@ -99,6 +99,21 @@ def test_against_64_bits(dtype):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("betas, lr, t", [
+    ((0.9, 0.999999), 1e-3, 12314), ((0.9, 0.999999), 1e-3, 155629),
+    ((0.99999, 0.999), 1e-4, 20739), ((0.999999, 0.999), 1e-3, 5943),
+    ((0.9, 0.999), 1e-3, 400000), ((0.9, 0.99999), 3e-4, 2 ** 31 - 2)])
+def test_bits_late_in_a_run(bits, betas, lr, t):
+    """At step counts and betas where the power's error decides a float32."""
+    cpu, gpu = pair([(4096,), (33,)], torch.float32, bits)
+    for _, _, opt in (cpu, gpu):
+        opt.betas = betas
+        opt.set_step(t - 1)
+        opt.step(lr)
+    same(cpu, gpu)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_many_tensors(bits):
     """More tensors than one launch's arguments hold."""
     cpu, gpu = pair([(i % 37 + 1,) for i in range(500)], torch.bfloat16, bits)
