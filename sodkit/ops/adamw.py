@@ -60,6 +60,21 @@ def _order(t: torch.Tensor) -> "tuple[int, ...]":
     return tuple(st if sz > 1 else 0 for st, sz in zip(t.stride(), t.shape))
 
 
+def _checked(betas, eps) -> "tuple[tuple[float, float], float]":
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError(f"betas must lie in [0, 1), got {betas}")
+    # as the step has it: a zero would make 0/0 of moments that are zero
+    if not torch.tensor(float(eps), dtype=torch.float32) > 0.0:
+        raise ValueError(f"eps must be positive in float32, got {eps}")
+    return (float(b1), float(b2)), float(eps)
+
+
+def _check_step(step) -> None:
+    if step < 0 or step >= 2 ** 31 - 1:
+        raise ValueError(f"step must lie in [0, 2^31 - 1), got {step}")
+
+
 class SodAdamW:
     """``param_groups``: dicts ``{"params": [...], "weight_decay": float}``, the
     decay defaulting to ``weight_decay``.  ``state_bits``: 32 or 8.
@@ -83,15 +98,9 @@ class SodAdamW:
     def __init__(self, param_groups, betas: "tuple[float, float]" = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 32, seed: int = 0):
-        b1, b2 = betas
-        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
-            raise ValueError(f"betas must lie in [0, 1), got {betas}")
-        if not eps > 0.0:
-            raise ValueError(f"eps must be positive, got {eps}")
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
-        self.betas = (float(b1), float(b2))
-        self.eps = float(eps)
+        self.betas, self.eps = _checked(betas, eps)
         self.state_bits = state_bits
         self.seed = int(seed) & 0xFFFFFFFF
         self.groups = []
@@ -306,8 +315,7 @@ class SodAdamW:
 
     def set_step(self, step: int) -> None:
         """Set every parameter's count of steps taken."""
-        if step < 0 or step >= 2 ** 31 - 1:
-            raise ValueError(f"step must lie in [0, 2^31 - 1), got {step}")
+        _check_step(step)
         self._steps = [int(step)] * len(self._params)
         if self._plan is not None:
             self._plan.set_steps(self._steps)
@@ -331,6 +339,7 @@ class SodAdamW:
                 f"checkpoint holds the states of {sd.get('kind', 'sgd')}"
                 + (f" in {sd['state_bits']} bits" if "state_bits" in sd else "")
                 + f", not of adamw in {self.state_bits} bits")
+        betas, eps = _checked(sd["betas"], sd["eps"])
         saved = sd["param_state"]
         if len(saved) != len(self._params) or len(sd["group_wd"]) != len(self.groups):
             raise ValueError(f"checkpoint holds {len(saved)} parameters in "
@@ -346,8 +355,9 @@ class SodAdamW:
             if self.state_bits == 8 and tuple(st["order"]) != _order(p):
                 raise ValueError(f"checkpoint's 8-bit state of parameter {k} is "
                                  f"of another memory layout")
-        self.betas, self.eps = tuple(sd["betas"]), sd["eps"]
-        self.seed = sd["seed"]
+            _check_step(st["step"])
+        self.betas, self.eps = betas, eps
+        self.seed = int(sd["seed"]) & 0xFFFFFFFF
         for p, st in zip(self._params, saved):
             for n, t in self.state[p].items():
                 t.copy_(st[n])

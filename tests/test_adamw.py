@@ -347,6 +347,40 @@ def test_refusals():
     assert SodAdamW([]).step(0.1) is None
 
 
+@pytest.mark.parametrize("eps", [1e-46, 7e-46, 0.0, -1e-8, math.nan])
+def test_eps_that_float32_makes_zero(eps):
+    """The step divides by root + eps in float32; moments that are zero have no
+    root to save it."""
+    p = torch.nn.Parameter(torch.ones(4))
+    with pytest.raises(ValueError, match="eps"):
+        SodAdamW([{"params": [p]}], eps=eps)
+    opt = SodAdamW([{"params": [p]}], eps=2e-45, weight_decay=0.0)  # a denormal is enough
+    p.grad = torch.zeros(4)
+    opt.step(0.1)
+    assert torch.equal(p, torch.ones(4))
+    sd = opt.state_dict()
+    other = SodAdamW([{"params": [torch.nn.Parameter(torch.zeros(4))]}])
+    with pytest.raises(ValueError, match="eps"):
+        other.load_state_dict({**sd, "eps": eps})
+
+
+def test_load_checks_before_it_writes():
+    p = torch.nn.Parameter(torch.ones(4))
+    opt = SodAdamW([{"params": [p]}])
+    p.grad = torch.ones(4)
+    opt.step(0.1)
+    sd = opt.state_dict()
+    other = SodAdamW([{"params": [torch.nn.Parameter(torch.ones(4))]}], betas=(0.8, 0.9))
+    bad = [{**sd, "betas": b} for b in ((1.0, 0.9), (0.9, 1.5), (math.nan, 0.9))]
+    bad += [{**sd, "param_state": [{**sd["param_state"][0], "step": t}]}
+            for t in (-1, 2 ** 31 - 1)]
+    for x in bad:
+        with pytest.raises(ValueError):
+            other.load_state_dict(x)
+        assert other.betas == (0.8, 0.9) and not other.exp_avg.any()
+        assert other.state_dict()["param_state"][0]["step"] == 0
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C
