@@ -46,6 +46,8 @@ def _in_storage(t: torch.Tensor) -> torch.Tensor:
 
 def _dense(t: torch.Tensor) -> bool:
     """Every element of one stretch of storage, each once."""
+    if t.numel() == 0:
+        return True
     want = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape)
                                if sz != 1):

@@ -114,6 +114,23 @@ def test_groups_scale_and_skip():
     check(ps[2].detach(), want[0], want[5], "scaled")
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shape", [(0,), (0, 3), (3, 0), (2, 0, 4)])
+def test_empty_parameters(bits, shape):
+    """Whatever their strides; their neighbours step as if alone."""
+    p, alone = (torch.nn.Parameter(torch.ones(5)) for _ in range(2))
+    e = torch.nn.Parameter(torch.empty(shape))
+    opt = SodAdamW([{"params": [e, p]}], state_bits=bits)
+    one = SodAdamW([{"params": [alone]}], state_bits=bits)
+    for q in (e, p, alone):
+        q.grad = torch.full_like(q, 0.5)
+    opt.step(0.1)
+    one.step(0.1)
+    assert torch.equal(p, alone)
+    again = SodAdamW([{"params": [e, p]}], state_bits=bits)
+    again.load_state_dict(opt.state_dict())
+
+
 def test_strided_parameters_and_gradients():
     """Parameters in another order than row by row, gradients in either."""
     g = torch.Generator().manual_seed(1)

@@ -124,6 +124,18 @@ def test_many_tensors(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_empty_parameters(bits):
+    cpu, gpu = pair([(3, 0), (5,), (2, 0, 4), (300,), (0, 3)], torch.bfloat16, bits)
+    for _ in range(2):
+        cpu[2].step(1e-2)
+        gpu[2].step(1e-2)
+    same(cpu, gpu)
+    only = SodAdamW([{"params": [torch.nn.Parameter(torch.empty(3, 0, device="cuda"))]}],
+                    state_bits=bits)
+    only.step(1e-2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_mixed_types_and_no_gradient(bits):
     ps = [torch.nn.Parameter(torch.randn(300, device="cuda").to(t)) for t in TYPES]
     qs = [torch.nn.Parameter(p.detach().cpu()) for p in ps]
