@@ -142,6 +142,9 @@ class SodSGD:
                 "group_wd": [g["weight_decay"] for g in self.groups]}
 
     def load_state_dict(self, sd: dict) -> None:
+        if sd.get("kind", "sgd") != "sgd":
+            raise ValueError(f"checkpoint holds the states of {sd['kind']}, "
+                             f"not of sgd")
         self.momentum = sd["momentum"]
         self.nesterov = sd["nesterov"]
         it = iter(sd["param_state"])

@@ -398,6 +398,18 @@ def test_load_checks_before_it_writes():
         assert other.state_dict()["param_state"][0]["step"] == 0
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_sgd_refuses_its_checkpoint(bits):
+    """With a message that says why, and before it moves anything."""
+    p = torch.nn.Parameter(torch.ones(4))
+    sgd = SodSGD([{"params": [p]}], momentum=0.7)
+    opt = SodAdamW([{"params": [p]}], state_bits=bits)
+    with pytest.raises(ValueError, match="adamw"):
+        sgd.load_state_dict(opt.state_dict())
+    assert sgd.momentum == 0.7
+    sgd.load_state_dict(sgd.state_dict())
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C
