@@ -597,8 +597,12 @@ class AdamWPlan {
         grads_.resize(T);
     }
 
-    // Decay and step counts are set in place: a captured step reads them.
+    // Decay and step counts are set in place: a captured step reads them.  They
+    // come from host memory, which a capture cannot read.
     void set_decay(std::vector<double> wd) {
+        c10::DeviceGuard guard(dev_);
+        TORCH_CHECK(!capturing(), "adamw: the weight decay has changed, which "
+                    "cannot be captured: call update_decay() before the capture");
         TORCH_CHECK(wd.size() == infos_.size());
         for (size_t i = 0; i < wd.size(); ++i) infos_[i].wd = wd[i];
         write_info();
@@ -613,6 +617,8 @@ class AdamWPlan {
 
     // steps taken of every tensor; synchronizes
     std::vector<int64_t> get_steps() const {
+        c10::DeviceGuard guard(dev_);
+        TORCH_CHECK(!capturing(), "adamw: step counts cannot be read in a capture");
         auto s = steps_.cpu();
         std::vector<int64_t> out;
         for (size_t i = 0; i < params_.size(); ++i)
@@ -621,6 +627,8 @@ class AdamWPlan {
     }
 
     void set_steps(std::vector<int64_t> steps) {
+        c10::DeviceGuard guard(dev_);
+        TORCH_CHECK(!capturing(), "adamw: step counts cannot be set in a capture");
         TORCH_CHECK(steps.size() == params_.size());
         auto s = torch::empty({n_chunks_}, torch::kInt32);
         for (size_t i = 0; i < params_.size(); ++i) {

@@ -95,7 +95,9 @@ class SodAdamW:
 
     A step may be captured into a graph; ``betas``, ``eps``, ``seed`` and host
     values of ``lr`` and ``grad_scale`` are then the capture's, the states, step
-    counts, decay and device scalars what they are at each replay."""
+    counts and device scalars what they are at each replay.  Decay is too, once
+    ``update_decay`` has handed a change of the groups' ``weight_decay`` over; an
+    eager step does that by itself, one in a capture refuses."""
 
     def __init__(self, param_groups, betas: "tuple[float, float]" = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -247,6 +249,17 @@ class SodAdamW:
             self._plan.set_steps(self._steps)
             self.grad_src = self._grad_src
 
+    def update_decay(self) -> None:
+        """Hand the groups' ``weight_decay`` to the device, where it changed:
+        replays of a captured step go by it from here on, in the order of the
+        current stream.  Not in a capture."""
+        if self._plan is None:
+            return
+        wd = [g["weight_decay"] for g in self.groups]
+        if wd != self._plan_wd:
+            self._plan.set_decay(self._decay())
+            self._plan_wd = wd
+
     def step(self, lr, grad_scale: float = 1.0,
              scale_t: "torch.Tensor | None" = None) -> None:
         """``lr`` and ``scale_t`` as in ``SodSGD.step``: ``scale_t``, a float32
@@ -261,10 +274,7 @@ class SodAdamW:
         if self._plan is None:
             self._step_cpu(lr, grad_scale, scale_t)
             return
-        wd = [g["weight_decay"] for g in self.groups]
-        if wd != self._plan_wd:
-            self._plan.set_decay(self._decay())
-            self._plan_wd = wd
+        self.update_decay()
         lr_t = _NONE
         if isinstance(lr, torch.Tensor):
             if lr.is_cuda:

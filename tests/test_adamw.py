@@ -410,6 +410,34 @@ def test_sgd_refuses_its_checkpoint(bits):
     sgd.load_state_dict(sgd.state_dict())
 
 
+def test_update_decay_hands_changes_over():
+    """The device's copy is written when a group's decay changed, and if that
+    fails it is not taken for written."""
+    class Plan:
+        calls, fail = [], False
+
+        def set_decay(self, wd):
+            if self.fail:
+                raise RuntimeError("in a capture")
+            self.calls.append(wd)
+
+    opt = SodAdamW([{"params": [torch.nn.Parameter(torch.ones(2)) for _ in range(2)]},
+                    {"params": [torch.nn.Parameter(torch.ones(2))], "weight_decay": 0.5}],
+                   weight_decay=0.1)
+    opt.update_decay()                          # nothing to do on the CPU
+    opt._plan, opt._plan_wd = Plan(), [0.1, 0.5]
+    opt.update_decay()
+    assert Plan.calls == []
+    opt.groups[1]["weight_decay"] = 0.0
+    Plan.fail = True
+    with pytest.raises(RuntimeError):
+        opt.update_decay()
+    Plan.fail = False
+    opt.update_decay()
+    opt.update_decay()
+    assert Plan.calls == [[0.1, 0.1, 0.0]]
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C

@@ -289,6 +289,54 @@ def test_captured_step(bits, eager_first):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_decay_that_changes_under_replays(bits):
+    cpu, gpu = pair([(5000,), (33,)], torch.bfloat16, bits)
+    (_, _, opt), (_, _, gopt) = cpu, gpu
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gopt.step(1e-2)
+    for wd in (0.1, 0.4, 0.4, 0.0):
+        for o in (opt, gopt):
+            o.groups[0]["weight_decay"] = wd
+            o.update_decay()
+        graph.replay()
+        opt.step(1e-2)
+        same(cpu, gpu)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_decay_that_changed_before_a_capture(bits):
+    """Refused, with nothing moved; after update_decay the capture has it."""
+    cpu, gpu = pair([(5000,), (33,)], torch.bfloat16, bits)
+    (_, _, opt), (_, _, gopt) = cpu, gpu
+    for o in (opt, gopt):
+        o.step(1e-2)
+        o.groups[0]["weight_decay"] = 0.4
+    torch.cuda.synchronize()
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="update_decay"):
+            gopt.step(1e-2)
+        with pytest.raises(RuntimeError, match="capture"):
+            gopt.set_step(3)
+        with pytest.raises(RuntimeError, match="capture"):
+            gopt.state_dict()
+        torch.zeros(1, device="cuda")           # a graph that is not empty
+    assert [s["step"] for s in gopt.state_dict()["param_state"]] == [1, 1]
+    same(cpu, gpu)
+    gopt.update_decay()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gopt.step(1e-2)
+    for _ in range(3):
+        graph.replay()
+        opt.step(1e-2)
+        same(cpu, gpu)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_other_stream(bits):
     cpu, gpu = pair([(70001,), (5,)], torch.bfloat16, bits)
     side = torch.cuda.Stream()
