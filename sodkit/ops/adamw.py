@@ -130,6 +130,7 @@ class SodAdamW:
             raise ValueError("parameters overlap in memory")
         self._shapes = [p.shape for p in self._params]
         self._strides = [p.stride() for p in self._params]
+        self._dtypes = [p.dtype for p in self._params]
         self._grad_src = None
         self._allocate()
         self._make_plan()
@@ -299,8 +300,9 @@ class SodAdamW:
             grad = (self._grad_src or {}).get(p)
             grad = p.grad if grad is None else grad
             grads.append(grad)
-            if p.shape != self._shapes[k] or p.stride() != self._strides[k]:
-                raise RuntimeError(f"parameter {k} has changed its size or "
+            if (p.shape != self._shapes[k] or p.stride() != self._strides[k]
+                    or p.dtype != self._dtypes[k]):
+                raise RuntimeError(f"parameter {k} has changed its size, type or "
                                    f"layout since the optimizer was made")
             if grad is not None and (
                     grad.layout != torch.strided or grad.shape != p.shape

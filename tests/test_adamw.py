@@ -438,6 +438,20 @@ def test_update_decay_hands_changes_over():
     assert Plan.calls == [[0.1, 0.1, 0.0]]
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_of_another_type_is_refused(bits):
+    """A float32 parameter is its own master: gone to 16 bits it would lose it."""
+    for old, new in ((torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16),
+                     (torch.bfloat16, torch.float32)):
+        p = torch.nn.Parameter(torch.ones(5, dtype=old))
+        opt = SodAdamW([{"params": [p]}], state_bits=bits)
+        p.data = p.data.to(new)
+        p.grad = torch.ones_like(p)
+        with pytest.raises(RuntimeError, match="type"):
+            opt.step(0.1)
+        assert torch.equal(p, torch.ones(5, dtype=new))
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C
