@@ -558,9 +558,11 @@ class AdamWPlan {
             I.master = master[i];
             I.wd = wd[i];
             I.dtype = type_code(p, "parameter");
-            layouts_.push_back({p.scalar_type(), {}});
-            if (!p.is_contiguous())
+            layouts_.push_back({p.scalar_type(), {}, {}});
+            if (!p.is_contiguous()) {
+                layouts_.back().sizes = p.sizes().vec();
                 layouts_.back().strides = p.strides().vec();
+            }
             long pad = (I.numel + BLOCK - 1) / BLOCK * BLOCK;
             TORCH_CHECK(I.state % BLOCK == 0 && I.state == places);
             places += pad;
@@ -712,7 +714,8 @@ class AdamWPlan {
             TORCH_CHECK(p.numel() == infos_[i].numel && p.device() == dev_ &&
                         p.scalar_type() == l.dtype &&
                         (l.strides.empty() ? p.is_contiguous()
-                                           : p.strides() == l.strides),
+                                           : p.sizes() == l.sizes &&
+                                             same_order(p, l.strides)),
                         "adamw: parameter ", i, " has changed its size, type, "
                         "device or layout since the optimizer was made");
             const auto &src = grads_[i];
@@ -724,7 +727,7 @@ class AdamWPlan {
                         "parameter ", i, " must be dense, of its size and on "
                         "its device");
             now[i].grad_dtype = type_code(g, "gradient");
-            if (!(l.strides.empty() && g.is_contiguous()) && !same_order(g, p)) {
+            if (!(l.strides.empty() && g.is_contiguous()) && !same_order(g, p.strides())) {
                 // elements are paired by their place in storage
                 copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
                                                       g.options()).copy_(g));
@@ -763,9 +766,9 @@ class AdamWPlan {
     }
 
     // elements of equal place in storage are equal elements
-    static bool same_order(const torch::Tensor &a, const torch::Tensor &b) {
-        for (int64_t d = 0; d < a.dim(); ++d)
-            if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    static bool same_order(const torch::Tensor &t, at::IntArrayRef strides) {
+        for (int64_t d = 0; d < t.dim(); ++d)
+            if (t.size(d) > 1 && t.stride(d) != strides[d]) return false;
         return true;
     }
 
@@ -782,10 +785,10 @@ class AdamWPlan {
     std::vector<torch::Tensor> moments_;
     std::vector<sodkit::aw::Info> infos_;
     // a parameter's order in storage, which is its states': contiguous (no
-    // strides kept) or these
+    // sizes and strides kept) or these
     struct Layout {
         at::ScalarType dtype;
-        std::vector<int64_t> strides;
+        std::vector<int64_t> sizes, strides;
     };
     std::vector<Layout> layouts_;
     std::vector<int64_t> first_;

@@ -129,7 +129,7 @@ class SodAdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters overlap in memory")
         self._shapes = [p.shape for p in self._params]
-        self._strides = [p.stride() for p in self._params]
+        self._orders = [_order(p) for p in self._params]
         self._dtypes = [p.dtype for p in self._params]
         self._grad_src = None
         self._allocate()
@@ -300,7 +300,7 @@ class SodAdamW:
             grad = (self._grad_src or {}).get(p)
             grad = p.grad if grad is None else grad
             grads.append(grad)
-            if (p.shape != self._shapes[k] or p.stride() != self._strides[k]
+            if (p.shape != self._shapes[k] or _order(p) != self._orders[k]
                     or p.dtype != self._dtypes[k]):
                 raise RuntimeError(f"parameter {k} has changed its size, type or "
                                    f"layout since the optimizer was made")

@@ -452,6 +452,21 @@ def test_a_parameter_of_another_type_is_refused(bits):
         assert torch.equal(p, torch.ones(5, dtype=new))
 
 
+@pytest.mark.parametrize("shape", [(4, 3, 1, 1), (1, 5, 2, 3), (2, 1, 3, 4)])
+def test_strides_of_single_elements_do_not_count(shape):
+    """The same order in storage under other strides is no change of layout."""
+    x = torch.arange(math.prod(shape)).float()
+    last = x.view(shape).clone().contiguous(memory_format=torch.channels_last)
+    p, q = torch.nn.Parameter(last.clone()), torch.nn.Parameter(last.clone())
+    opts = [SodAdamW([{"params": [t]}]) for t in (p, q)]
+    strides = [st if n > 1 else 17 for st, n in zip(q.stride(), shape)]
+    q.data = q.data.as_strided(shape, strides)
+    for t, o in zip((p, q), opts):
+        t.grad = last * 0.1
+        o.step(0.1)
+    assert torch.equal(p, q) and not torch.equal(p, last)
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C

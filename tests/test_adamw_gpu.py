@@ -169,6 +169,34 @@ def test_layouts(bits):
         same(([ps[0]], None, opts[0]), ([ps[1]], None, opts[1]))
 
 
+@pytest.mark.parametrize("shape", [(4, 3, 1, 1), (1, 5, 2, 3), (2, 1, 3, 4)])
+def test_strides_of_single_elements_do_not_count(shape):
+    """The same order in storage under other strides is no change of layout."""
+    x = torch.arange(math.prod(shape), device="cuda").float()
+    last = x.view(shape).clone().contiguous(memory_format=torch.channels_last)
+    p, q = torch.nn.Parameter(last.clone()), torch.nn.Parameter(last.clone())
+    opts = [SodAdamW([{"params": [t]}]) for t in (p, q)]
+    strides = [st if n > 1 else 17 for st, n in zip(q.stride(), shape)]
+    q.data = q.data.as_strided(shape, strides)
+    for t, o in zip((p, q), opts):
+        t.grad = last * 0.1
+        o.step(0.1)
+    assert torch.equal(p, q) and not torch.equal(p, last)
+
+
+def test_another_size_in_the_same_strides_is_refused():
+    p = torch.nn.Parameter(torch.ones(6, 4, device="cuda").t())
+    opt = SodAdamW([{"params": [p]}])
+    wide = torch.ones(31, device="cuda")
+    for shape, strides in (((3, 8), (1, 4)), ((24,), (1,)), ((2, 3, 4), (1, 2, 6))):
+        p.data = wide.as_strided(shape, strides)
+        p.grad = None
+        opt.grad_src = {p: torch.ones(shape, device="cuda")}
+        with pytest.raises(RuntimeError, match="changed"):
+            opt.step(0.1)
+    assert (wide == 1).all()
+
+
 def test_decay_that_changes():
     cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
     for wd in (0.1, 0.4):
