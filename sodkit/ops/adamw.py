@@ -267,6 +267,9 @@ class SodAdamW:
         scalar on the parameters' device, is multiplied into ``grad_scale``
         and skips the whole step where it is 0; ``lr`` may be a device float32
         scalar, which a captured step reads anew on each replay."""
+        for what, t in (("lr", lr), ("scale_t", scale_t)):
+            if isinstance(t, torch.Tensor) and t.numel() != 1:
+                raise RuntimeError(f"{what} must be a scalar, got {tuple(t.shape)}")
         if not self._params:
             return
         if self._params[0].device != self._master.device:

@@ -530,6 +530,24 @@ def test_refusals():
         SodAdamW([{"params": [p, torch.nn.Parameter(torch.ones(3))]}])
 
 
+@pytest.mark.parametrize("shape", [(0,), (2,), (3, 1)])
+def test_scalars_that_are_none(shape):
+    """An empty one is not taken for one that was not given."""
+    p = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = SodAdamW([{"params": [p]}])
+    t, one = torch.ones(shape, device="cuda"), torch.ones((), device="cuda")
+    with pytest.raises(RuntimeError, match="lr must be"):
+        opt.step(t)
+    with pytest.raises(RuntimeError, match="scale_t must be"):
+        opt.step(0.1, scale_t=t)
+    for kw in (dict(loss_scale=t), dict(loss_scale=one, good_steps=t, skips=one),
+               dict(loss_scale=one, good_steps=one, skips=t)):
+        with pytest.raises(ValueError, match="must be a scalar"):
+            grad_norm([p.grad], **kw)
+    assert (p == 1).all()
+
+
 # ------------------------------------------------------------------ the norm
 
 @pytest.mark.parametrize("dtype", TYPES)
