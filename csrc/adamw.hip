@@ -720,6 +720,8 @@ class AdamWPlan {
                         "device or layout since the optimizer was made");
             const auto &src = grads_[i];
             const auto &g = src.defined() && src.numel() ? src : p.grad();
+            TORCH_CHECK(in_memory(p), "adamw: parameter ", i,
+                        " has no memory");
             now[i] = {p.data_ptr(), nullptr, 0};
             if (!g.defined()) continue;
             TORCH_CHECK(g.layout() == torch::kStrided && g.device() == dev_ &&
@@ -727,7 +729,12 @@ class AdamWPlan {
                         "parameter ", i, " must be dense, of its size and on "
                         "its device");
             now[i].grad_dtype = type_code(g, "gradient");
-            if (!(l.strides.empty() && g.is_contiguous()) && !same_order(g, p.strides())) {
+            bool same = (l.strides.empty() && g.is_contiguous()) ||
+                        same_order(g, p.strides());
+            TORCH_CHECK(same ? in_memory(g) : g.storage().nbytes() != 0,
+                        "adamw: the gradient of parameter ", i,
+                        " has no memory");
+            if (!same) {
                 // elements are paired by their place in storage
                 copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
                                                       g.options()).copy_(g));
@@ -763,6 +770,14 @@ class AdamWPlan {
             made_on_ = stream;
         }
         return rows;
+    }
+
+    // a dense tensor's storage holds it (it may have been resized, or never
+    // been there)
+    static bool in_memory(const torch::Tensor &t) {
+        return t.numel() == 0 ||
+               t.storage().nbytes() >=
+                   (size_t)((t.storage_offset() + t.numel()) * t.element_size());
     }
 
     // elements of equal place in storage are equal elements

@@ -282,7 +282,11 @@ std::vector<torch::Tensor> grad_norm(pybind11::list list, double prescale,
                     "float32, bfloat16 or float16, got ", t);
         codes[i] = t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : 2;
         // the order of the elements is of no consequence, holes and overlaps are
-        if (!g.is_non_overlapping_and_dense()) {
+        bool dense = g.is_non_overlapping_and_dense();
+        size_t ends = dense ? (g.storage_offset() + g.numel()) * g.element_size() : 1;
+        TORCH_CHECK(g.numel() == 0 || g.storage().nbytes() >= ends,
+                    "grad_norm: gradient ", i, " has no memory");
+        if (!dense) {
             copies.push_back(g.contiguous());
             grads[i] = &copies.back();
         }

@@ -197,6 +197,31 @@ def test_another_size_in_the_same_strides_is_refused():
     assert (wide == 1).all()
 
 
+def test_no_memory_is_refused():
+    """Storage that was given back, or never there, is not read."""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = SodAdamW([{"params": [p]}])
+    for gone in (torch.ones(300, device="cuda"), torch.ones(400, device="cuda")[50:350],
+                 torch.ones(600, device="cuda")[::2]):
+        gone.untyped_storage().resize_(0)
+        opt.grad_src = {p: gone}
+        with pytest.raises(RuntimeError, match="no memory"):
+            opt.step(0.1)
+        with pytest.raises(RuntimeError, match="no memory"):
+            grad_norm([gone])
+    part = torch.ones(300, device="cuda")
+    part.untyped_storage().resize_(299 * 4)
+    opt.grad_src = {p: part}
+    with pytest.raises(RuntimeError, match="no memory"):
+        opt.step(0.1)
+    with pytest.raises(RuntimeError, match="no memory"):
+        grad_norm([torch.ones(5, device="cuda"), part])
+    opt.grad_src = {p: torch.ones(300, device="cuda")}
+    p.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="no memory"):
+        opt.step(0.1)
+
+
 def test_decay_that_changes():
     cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
     for wd in (0.1, 0.4):
