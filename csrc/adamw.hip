@@ -722,6 +722,7 @@ class AdamWPlan {
             const auto &g = src.defined() && src.numel() ? src : p.grad();
             TORCH_CHECK(in_memory(p), "adamw: parameter ", i,
                         " has no memory");
+            TORCH_CHECK(!p.is_neg(), "adamw: parameter ", i, " is a negated view");
             now[i] = {p.data_ptr(), nullptr, 0};
             if (!g.defined()) continue;
             TORCH_CHECK(g.layout() == torch::kStrided && g.device() == dev_ &&
@@ -734,8 +735,9 @@ class AdamWPlan {
             TORCH_CHECK(same ? in_memory(g) : g.storage().nbytes() != 0,
                         "adamw: the gradient of parameter ", i,
                         " has no memory");
-            if (!same) {
-                // elements are paired by their place in storage
+            if (!same || g.is_neg()) {
+                // elements are paired by their place in storage, and a view
+                // that stands for its negation is read without the sign
                 copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
                                                       g.options()).copy_(g));
                 now[i].grad = copies.back().data_ptr();

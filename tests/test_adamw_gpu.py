@@ -222,6 +222,28 @@ def test_no_memory_is_refused():
         opt.step(0.1)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_negated_views(bits):
+    """A view that stands for the negation of its memory counts with its sign."""
+    x = torch.randn(300)
+    c = torch.complex(torch.zeros(1), torch.ones(1))
+    for n, view in ((300, lambda d: torch._neg_view(x.to(d))),
+                    (1, lambda d: c.to(d).conj().imag)):
+        sides = []
+        for d in ("cpu", "cuda"):
+            p = torch.nn.Parameter(torch.ones(n, device=d))
+            opt = SodAdamW([{"params": [p]}], state_bits=bits)
+            g = view(d)
+            assert g.is_neg() and g.is_contiguous()
+            opt.grad_src = {p: g}
+            opt.step(1e-2)
+            sides.append(([p], None, opt))
+        same(*sides)
+    p.data = torch._neg_view(p.data)
+    with pytest.raises(RuntimeError, match="negated"):
+        opt.step(1e-2)
+
+
 def test_decay_that_changes():
     cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
     for wd in (0.1, 0.4):
