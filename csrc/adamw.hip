@@ -751,6 +751,7 @@ class AdamWPlan {
                                                 stream.id()));
             return rows_;
         }
+        check_apart(now);
         // A table that a graph reads is never written again, and one that is
         // made in a capture belongs to the graph alone.
         auto rows = torch::empty(
@@ -772,6 +773,27 @@ class AdamWPlan {
             made_on_ = stream;
         }
         return rows;
+    }
+
+    // Two workgroups may not step the same memory.  Looked at where parameters
+    // moved since the last look.
+    void check_apart(const std::vector<Row> &now) {
+        bool moved = apart_.size() != now.size();
+        for (size_t i = 0; !moved && i < now.size(); ++i)
+            moved = apart_[i] != now[i].param;
+        if (!moved) return;
+        std::vector<std::pair<const char *, const char *>> spans;
+        for (size_t i = 0; i < now.size(); ++i) {
+            auto *p = static_cast<const char *>(now[i].param);
+            size_t n = params_[i].numel() * params_[i].element_size();
+            if (n) spans.push_back({p, p + n});
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            TORCH_CHECK(spans[i - 1].second <= spans[i].first,
+                        "adamw: parameters overlap in memory");
+        apart_.resize(now.size());
+        for (size_t i = 0; i < now.size(); ++i) apart_[i] = now[i].param;
     }
 
     // a dense tensor's storage holds it (it may have been resized, or never
@@ -812,6 +834,7 @@ class AdamWPlan {
     int64_t n_chunks_ = 0;
     torch::Tensor info_, chunks_, steps_, rows_;
     std::vector<Row> host_, now_;           // rows_' content; this step's
+    std::vector<const void *> apart_;       // parameters that do not overlap
     bool kept_ = false;                     // a captured graph reads rows_
     std::vector<torch::Tensor> graphs_;     // tables that graphs read
     // the streams that the states and that rows_ were allocated on

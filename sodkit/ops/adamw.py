@@ -124,16 +124,25 @@ class SodAdamW:
             if not _dense(p):
                 raise ValueError("parameters must be dense and without "
                                  f"overlaps, got strides {p.stride()} of {tuple(p.shape)}")
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
-                       for p in self._params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise ValueError("parameters overlap in memory")
+        self._looked_at = None
+        self._check_apart(ValueError)
         self._shapes = [p.shape for p in self._params]
         self._orders = [_order(p) for p in self._params]
         self._dtypes = [p.dtype for p in self._params]
         self._grad_src = None
         self._allocate()
         self._make_plan()
+
+    def _check_apart(self, error) -> None:
+        """Where no parameter moved since the last look, nothing is done."""
+        at = [p.data_ptr() for p in self._params]
+        if at == self._looked_at:
+            return
+        spans = sorted((a, a + p.numel() * p.element_size())
+                       for a, p in zip(at, self._params) if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise error("parameters overlap in memory")
+        self._looked_at = at
 
     def _allocate(self) -> None:
         dev = self._params[0].device if self._params else torch.device("cpu")
@@ -313,6 +322,7 @@ class SodAdamW:
                 raise RuntimeError(
                     f"the gradient of parameter {k} must be dense, of its "
                     f"size, on its device and float32, bfloat16 or float16")
+        self._check_apart(RuntimeError)
         for k, (p, grad, wd) in enumerate(zip(self._params, grads, self._decay())):
             if grad is None or p.numel() == 0:
                 continue

@@ -485,6 +485,25 @@ def test_scalars_that_are_none(shape):
     assert (p == 1).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_come_to_overlap(bits):
+    """Weights that move are looked at again; apart again, they step."""
+    flat = torch.ones(600)
+    ps = [torch.nn.Parameter(flat[:300]), torch.nn.Parameter(flat[300:])]
+    opt = SodAdamW([{"params": ps}], state_bits=bits)
+    opt.grad_src = {p: torch.ones(300) for p in ps}
+    opt.step(0.1)
+    for tied in (flat[:300], flat[299:599]):
+        before = flat.clone()
+        ps[1].data = tied
+        with pytest.raises(RuntimeError, match="overlap"):
+            opt.step(0.1)
+        assert torch.equal(flat, before)
+        ps[1].data = flat[300:]
+        opt.step(0.1)
+        assert not torch.equal(flat, before)
+
+
 def test_native_refusals():
     """The extension's own checks, which a GPU call would reach."""
     from sodkit import _C

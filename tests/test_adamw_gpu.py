@@ -244,6 +244,25 @@ def test_negated_views(bits):
         opt.step(1e-2)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_that_come_to_overlap(bits):
+    """Weights that move are looked at again; apart again, they step."""
+    flat = torch.ones(600, device="cuda")
+    ps = [torch.nn.Parameter(flat[:300]), torch.nn.Parameter(flat[300:])]
+    opt = SodAdamW([{"params": ps}], state_bits=bits)
+    opt.grad_src = {p: torch.ones(300, device="cuda") for p in ps}
+    opt.step(0.1)
+    for tied in (flat[:300], flat[299:599]):
+        before = flat.clone()
+        ps[1].data = tied
+        with pytest.raises(RuntimeError, match="overlap"):
+            opt.step(0.1)
+        assert torch.equal(flat, before)
+        ps[1].data = flat[300:]
+        opt.step(0.1)
+        assert not torch.equal(flat, before)
+
+
 def test_decay_that_changes():
     cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
     for wd in (0.1, 0.4):
