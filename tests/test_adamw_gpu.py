@@ -558,6 +558,30 @@ def test_past_32_bits():
     assert abs(norm.item() - want) <= 2.0 ** -23 * want
 
 
+def test_past_32_bits_with_32_bit_moments():
+    """The same with moments in 32 bits."""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    n = 2 ** 32 + 300
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    opt = SodAdamW([{"params": [p], "weight_decay": 0.1}])
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    head, tail = torch.randn(300).bfloat16(), torch.randn(300).bfloat16()
+    g[:300], g[-300:] = head.cuda(), tail.cuda()
+    p.grad = g
+    opt.step(1e-2)
+    for part, grad in ((slice(0, 300), head), (slice(n - 300, n), tail)):
+        q = torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16))
+        q.grad = grad
+        one = SodAdamW([{"params": [q], "weight_decay": 0.1}])
+        one.step(1e-2)
+        assert differ(p[part], q) == 0
+        for a, b in ((opt.master, one.master), (opt.exp_avg, one.exp_avg),
+                     (opt.exp_avg_sq, one.exp_avg_sq)):
+            assert differ(a[part], b[:300]) == 0
+    assert not opt.exp_avg[300:n - 300].any() and not p[300:n - 300].any()
+
+
 def test_refusals():
     p = torch.nn.Parameter(torch.ones(4, device="cuda"))
     opt = SodAdamW([{"params": [p]}])
@@ -647,6 +671,82 @@ def test_grad_norm_ends(dtype, n):
         want = 2.0 * math.sqrt(part.numel())
         assert abs(norm - want) <= 2.0 ** -23 * want
         part.zero_()
+
+
+def apart(sizes, dtypes, fill=None):
+    """Gradients with a NaN between them, so that no two are neighbours and
+    nothing beside them may be read, of the types in turn."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    ends = [0] * len(dtypes)
+    places = []
+    for k, n in enumerate(sizes):
+        places.append(ends[k % len(dtypes)] + 1)
+        ends[k % len(dtypes)] += n + 1
+    flats = [torch.full((e + 1,), math.nan, dtype=t, device="cuda")
+             for e, t in zip(ends, dtypes)]
+    out = []
+    for k, n in enumerate(sizes):
+        g = flats[k % len(dtypes)][places[k]:places[k] + n]
+        g.copy_(torch.randint(-3, 4, (n,), device="cuda", generator=gen)
+                if fill is None else torch.full((n,), fill, device="cuda"))
+        out.append(g)
+    return out
+
+
+def merged(grads):
+    """How many stretches of memory they are."""
+    return 1 + sum(a.dtype != b.dtype or a.data_ptr() + a.numel() * a.element_size()
+                   != b.data_ptr() for a, b in zip(grads, grads[1:]))
+
+
+@pytest.mark.parametrize("count", [1, 5, 64, 159, 160, 161, 320, 321, 700])
+@pytest.mark.parametrize("size", [1, 23, 103, 8192, 8193, 20000])
+@pytest.mark.parametrize("dtypes", [TYPES[:1], TYPES[1:2], TYPES])
+def test_grad_norm_apart(count, size, dtypes):
+    """Tensors that lie apart, below and past what one launch takes, in total and in
+    number.  Whole numbers: the sum in 64 bits is exact, whatever its order, and
+    the root is rounded once to 64 and once to 32 bits."""
+    sizes = [max(1, size - 3 * (k % 7)) for k in range(count)]
+    grads = apart(sizes, dtypes)
+    assert merged(grads) == count
+    total = sum(int(g.double().square().sum().item()) for g in grads)
+    norm, mult = grad_norm(grads, max_norm=1.0)
+    assert norm.item() == torch.tensor(math.sqrt(total)).float().item()
+    again = grad_norm(grads, max_norm=1.0)
+    assert norm.item() == again[0].item() and mult.item() == again[1].item()
+
+
+@pytest.mark.parametrize("count, size", [(5, 7), (160, 100), (160, 9000), (161, 3), (700, 8200)])
+def test_grad_norm_apart_ends(count, size):
+    """The first and the last element of every tensor that ends or starts a launch's
+    share count, alone."""
+    grads = apart([size] * count, TYPES, fill=0.0)
+    for k in sorted({0, 1, count // 2, count - 1, *(k for k in (63, 64, 159, 160, 319, 320, 639)
+                                                    if k < count)}):
+        for i in (0, size - 1):
+            grads[k][i] = 2.0
+            assert grad_norm(grads)[0].item() == 2.0, (k, i)
+            grads[k][i] = 0.0
+
+
+def test_grad_norm_apart_captured():
+    """Several launches and the scaler in a graph, eager work between the replays."""
+    grads = apart([8193, 5, 300] * 150, TYPES)
+    scale, good, skips = (torch.tensor(v, device="cuda") for v in (8.0, 0.0, 0.0))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm, mult = grad_norm(grads, max_norm=1.0, loss_scale=scale,
+                               good_steps=good, skips=skips, growth_interval=2)
+    for i in range(4):
+        for g in grads[::40]:
+            g.fill_(i)
+        before = scale.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = grad_norm(grads, max_norm=1.0, loss_scale=before)
+        assert differ(norm, want[0]) == 0 and differ(mult, want[1]) == 0
+        assert math.isfinite(norm.item()) and scale.item() == 8.0 * 2 ** ((i + 1) // 2)
 
 
 def test_grad_norm_views_and_range():
