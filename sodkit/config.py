@@ -45,7 +45,7 @@ class Config:
     adam_eps: float = 1e-8
     adam_state_bits: int = 32            # 32 | 8 (stochastically rounded codes)
     epoch_num: int = 3
-    lr: float = 0.05
+    lr: float = 0.05                     # SGD's, in the presets too; adamw: 1e-4 to 1e-3
     momentum: float = 0.9
     weight_decay: float = 5e-4
     nesterov: bool = False

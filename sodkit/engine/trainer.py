@@ -86,6 +86,9 @@ class Solver:
                 groups, betas=(cfg.adam_beta1, cfg.adam_beta2),
                 eps=cfg.adam_eps, weight_decay=cfg.weight_decay,
                 state_bits=cfg.adam_state_bits, seed=cfg.seed)
+            if cfg.lr >= 0.01:      # the presets' rates are SGD's
+                self.log.info(f"lr {cfg.lr:g} is a rate for SGD: AdamW moves a "
+                              f"weight by about lr a step, 1e-4 to 1e-3 is usual")
         elif cfg.optimizer == "sgd":
             self.optimizer = ops.SodSGD(groups, momentum=cfg.momentum,
                                         weight_decay=cfg.weight_decay,

@@ -689,6 +689,17 @@ def test_solver_device_scaler_state(tmp_path):
     assert (s._scale_t.item(), s._skips_t.item()) == (64.0, 1.0)
 
 
+def test_solver_says_when_the_rate_is_sgds(tmp_path):
+    """AdamW with a rate that was left as it is for SGD says so, any other is quiet."""
+    for k, (kw, said) in enumerate(((dict(optimizer="adamw"), True),
+                                    (dict(optimizer="adamw", lr=1e-3), False),
+                                    (dict(), False))):
+        s = Solver(make_config("cpu_plumbing", output_root=str(tmp_path),
+                               exp_name=f"e{k}", **kw))
+        with open(s.paths["log"]) as f:
+            assert ("a rate for SGD" in f.read()) == said
+
+
 def test_unknown_optimizer(tmp_path):
     with pytest.raises(ValueError, match="optimizer"):
         Solver(make_config("cpu_plumbing", output_root=str(tmp_path), optimizer="adam"))
