@@ -435,6 +435,10 @@ __global__ void bn_bwd_reduce_kernel(const T *__restrict__ dy,
 }
 
 // ---- vectorized backward apply (C % 8 == 0) ----
+// The float16 form with mask and residual gradient would take 71 registers and
+// keeps one of them in scratch memory: 454 us against 508 with 7 waves for
+// [64, 256, 128, 128], 103 against 104 for [32, 256, 88, 88], but 44.6 against
+// 42.5, 22.9 against 22.0 and 13.4 against 12.6 for that one's next three stages.
 template <typename T, bool RELU, bool NEED_DRES, bool MASKED>
 __global__ void __launch_bounds__(256, 8)     // 64 registers: 8 waves a SIMD
 bn_bwd_apply_vec_kernel(const T *__restrict__ dy,
