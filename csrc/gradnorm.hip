@@ -307,23 +307,31 @@ std::vector<torch::Tensor> grad_norm(pybind11::list list, double prescale,
     f.mult = mult.data_ptr<float>();
 
     auto stream = at::hip::getCurrentHIPStream().stream();
-    // Neighbours in memory (the views of a bucket) are one stretch.
-    struct Stretch { const char *ptr; long numel; unsigned char dtype; };
+    // Neighbours in one storage (the views of a bucket) are one stretch.  Those
+    // of two storages are not: how the sum is grouped, and so its last bits,
+    // would hang on where the allocator put them, on every rank elsewhere.
+    struct Stretch {
+        const char *ptr;
+        long numel;
+        unsigned char dtype;
+        const c10::StorageImpl *storage;
+    };
     std::vector<Stretch> parts;
     parts.reserve(T);
     for (size_t i = 0; i < T; ++i) {
         long n = grads[i]->numel();
         if (n == 0) continue;
         const char *p = static_cast<const char *>(grads[i]->data_ptr());
+        const auto *storage = grads[i]->storage().unsafeGetStorageImpl();
         if (!parts.empty()) {
             auto &l = parts.back();
-            if (l.dtype == codes[i] &&
+            if (l.storage == storage && l.dtype == codes[i] &&
                 l.ptr + l.numel * (codes[i] == 0 ? 4 : 2) == p) {
                 l.numel += n;
                 continue;
             }
         }
-        parts.push_back({p, n, codes[i]});
+        parts.push_back({p, n, codes[i], storage});
     }
     const size_t N = parts.size(), n_launch = std::max<size_t>(1, (N + SEGS - 1) / SEGS);
     torch::Tensor partial;

@@ -37,8 +37,9 @@ def grad_norm(grads: Sequence[torch.Tensor], prescale: float = 1.0,
     ``mult`` is of the scale before.
 
     Gradients may be float32, bfloat16 and float16, mixed, with any strides,
-    on one device.  The sum is held in 64 bits and a repeated call gives the
-    same bits."""
+    on one device.  The sum is held in 64 bits, and how it is grouped goes by the
+    sizes and by which gradients are neighbours in one storage, not by
+    addresses: a repeated call, and every rank, gets the same bits."""
     if not isinstance(grads, list):
         grads = list(grads)
     if not grads:

@@ -729,6 +729,23 @@ def test_grad_norm_apart_ends(count, size):
             grads[k][i] = 0.0
 
 
+def test_grad_norm_wherever_the_allocator_puts_it():
+    """Two tensors beside each other and the same two apart: the same bits.  The sum
+    of squares is 2^46 + 2^23 + 1/4, whose root lies half way between two float32,
+    and 15 squares of 2^-8 that decide it unless each is added to 2^46 by itself."""
+    flat = torch.zeros(8192, device="cuda")
+    flat[0], flat[4096], flat[4097], flat[4098] = 2.0 ** 23, 2.0 ** 11, 2.0 ** 11, 0.5
+    flat[256:4096:256] = 2.0 ** -4
+    rest = torch.zeros(20000, device="cuda")    # more than one workgroup's
+    near = [torch.from_dlpack(flat[:4096]), torch.from_dlpack(flat[4096:])]
+    assert near[0].data_ptr() + 4096 * 4 == near[1].data_ptr()
+    gap = torch.zeros(3, 4096, device="cuda")
+    far = [gap[0].copy_(flat[:4096]), gap[2].copy_(flat[4096:])]
+    assert [grad_norm(x + [rest])[0].item() for x in (near, far)] == [2.0 ** 23] * 2
+    # one stretch of one storage: grouped otherwise
+    assert grad_norm([*flat.split(4096), rest])[0].item() == 2.0 ** 23 + 1
+
+
 def test_grad_norm_apart_captured():
     """Several launches and the scaler in a graph, eager work between the replays."""
     grads = apart([8193, 5, 300] * 150, TYPES)
