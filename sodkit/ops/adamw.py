@@ -23,7 +23,8 @@ CPU path: ops.reference.adamw_step / adamw8_step, the same operations.
 
 from __future__ import annotations
 
-from typing import Iterable
+from types import MappingProxyType
+from typing import Iterable, Mapping
 
 import torch
 
@@ -233,13 +234,14 @@ class SodAdamW:
     # step, and the reducer's gather lands it in the stable bucket views given
     # here.  Without them a gradient that moved is seen, at the price of a new
     # table in front of the step.
+    # What is given is taken as it is now; to change it, give another.
     @property
-    def grad_src(self) -> "dict[torch.nn.Parameter, torch.Tensor] | None":
+    def grad_src(self) -> "Mapping[torch.nn.Parameter, torch.Tensor] | None":
         return self._grad_src
 
     @grad_src.setter
     def grad_src(self, views) -> None:
-        self._grad_src = views
+        self._grad_src = None if views is None else MappingProxyType(dict(views))
         if self._plan is not None:
             views = views or {}
             self._plan.set_grads([views.get(p, _NONE) for p in self._params])

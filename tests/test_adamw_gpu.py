@@ -263,6 +263,24 @@ def test_parameters_that_come_to_overlap(bits):
         assert not torch.equal(flat, before)
 
 
+def test_grad_src_is_what_was_given():
+    """Neither path goes by what becomes of the dict later, and the optimizer's own
+    cannot be written."""
+    p = torch.nn.Parameter(torch.zeros(3, device="cuda"))
+    opt = SodAdamW([{"params": [p]}])
+    views = {p: torch.ones(3, device="cuda")}
+    opt.grad_src = views
+    views[p] = -views[p]
+    opt.step(0.1)
+    assert (p < 0).all()
+    with pytest.raises(TypeError):
+        opt.grad_src[p] = views[p]
+    opt.grad_src = {**opt.grad_src, p: views[p]}
+    for _ in range(3):
+        opt.step(0.1)
+    assert (p > 0).all()
+
+
 def test_decay_that_changes():
     cpu, gpu = pair([(500,), (33,)], torch.float32, 32)
     for wd in (0.1, 0.4):
