@@ -718,10 +718,7 @@ class AdamWPlan {
                                              same_order(p, l.strides)),
                         "adamw: parameter ", i, " has changed its size, type, "
                         "device or layout since the optimizer was made");
-            const auto &src = grads_[i];
-            const auto &g = src.defined() && src.numel() ? src : p.grad();
-            TORCH_CHECK(in_memory(p), "adamw: parameter ", i,
-                        " has no memory");
+            const auto &g = gradient(i);
             TORCH_CHECK(!p.is_neg(), "adamw: parameter ", i, " is a negated view");
             now[i] = {p.data_ptr(), nullptr, 0};
             if (!g.defined()) continue;
@@ -732,10 +729,10 @@ class AdamWPlan {
             now[i].grad_dtype = type_code(g, "gradient");
             bool same = (l.strides.empty() && g.is_contiguous()) ||
                         same_order(g, p.strides());
-            TORCH_CHECK(same ? in_memory(g) : g.storage().nbytes() != 0,
-                        "adamw: the gradient of parameter ", i,
-                        " has no memory");
             if (!same || g.is_neg()) {
+                TORCH_CHECK(g.numel() == 0 || g.storage().nbytes() != 0,
+                            "adamw: the gradient of parameter ", i,
+                            " has no memory");
                 // elements are paired by their place in storage, and a view
                 // that stands for its negation is read without the sign
                 copies.push_back(torch::empty_strided(p.sizes(), p.strides(),
@@ -751,6 +748,7 @@ class AdamWPlan {
                                                 stream.id()));
             return rows_;
         }
+        check_memory(now);
         check_apart(now);
         // A table that a graph reads is never written again, and one that is
         // made in a capture belongs to the graph alone.
@@ -796,12 +794,26 @@ class AdamWPlan {
         for (size_t i = 0; i < now.size(); ++i) apart_[i] = now[i].param;
     }
 
-    // a dense tensor's storage holds it (it may have been resized, or never
-    // been there)
-    static bool in_memory(const torch::Tensor &t) {
-        return t.numel() == 0 ||
-               t.storage().nbytes() >=
-                   (size_t)((t.storage_offset() + t.numel()) * t.element_size());
+    // Storages may have been resized, or never been there.  An address that
+    // was looked at before is good: another size has another.
+    void check_memory(const std::vector<Row> &now) const {
+        auto held = [](const torch::Tensor &t) {
+            return t.numel() == 0 ||
+                   t.storage().nbytes() >= (size_t)((t.storage_offset() + t.numel()) *
+                                                    t.element_size());
+        };
+        for (size_t i = 0; i < now.size(); ++i) {
+            if (i < host_.size() && now[i] == host_[i]) continue;
+            const auto &p = params_[i], &g = gradient(i);
+            TORCH_CHECK(held(p), "adamw: parameter ", i, " has no memory");
+            TORCH_CHECK(!g.defined() || !same_order(g, p.strides()) || held(g),
+                        "adamw: the gradient of parameter ", i, " has no memory");
+        }
+    }
+
+    const torch::Tensor &gradient(size_t i) const {
+        const auto &src = grads_[i];
+        return src.defined() && src.numel() ? src : params_[i].grad();
     }
 
     // elements of equal place in storage are equal elements

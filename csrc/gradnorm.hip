@@ -282,11 +282,9 @@ std::vector<torch::Tensor> grad_norm(pybind11::list list, double prescale,
                     "float32, bfloat16 or float16, got ", t);
         codes[i] = t == torch::kFloat32 ? 0 : t == torch::kBFloat16 ? 1 : 2;
         // the order of the elements is of no consequence, holes and overlaps are
-        bool dense = g.is_non_overlapping_and_dense();
-        size_t ends = dense ? (g.storage_offset() + g.numel()) * g.element_size() : 1;
-        TORCH_CHECK(g.numel() == 0 || g.storage().nbytes() >= ends,
-                    "grad_norm: gradient ", i, " has no memory");
-        if (!dense) {
+        if (!g.is_non_overlapping_and_dense()) {
+            TORCH_CHECK(g.numel() == 0 || g.storage().nbytes() != 0,
+                        "grad_norm: gradient ", i, " has no memory");
             copies.push_back(g.contiguous());
             grads[i] = &copies.back();
         }
@@ -333,6 +331,11 @@ std::vector<torch::Tensor> grad_norm(pybind11::list list, double prescale,
         }
         parts.push_back({p, n, codes[i], storage});
     }
+    for (const auto &p : parts)     // a storage may have been resized
+        TORCH_CHECK(p.ptr + p.numel * (p.dtype == 0 ? 4 : 2) <=
+                        static_cast<const char *>(p.storage->data()) +
+                            p.storage->nbytes(),
+                    "grad_norm: a gradient has no memory");
     const size_t N = parts.size(), n_launch = std::max<size_t>(1, (N + SEGS - 1) / SEGS);
     torch::Tensor partial;
     double *out = nullptr;

@@ -278,9 +278,10 @@ class SodAdamW:
         scalar on the parameters' device, is multiplied into ``grad_scale``
         and skips the whole step where it is 0; ``lr`` may be a device float32
         scalar, which a captured step reads anew on each replay."""
-        for what, t in (("lr", lr), ("scale_t", scale_t)):
-            if isinstance(t, torch.Tensor) and t.numel() != 1:
-                raise RuntimeError(f"{what} must be a scalar, got {tuple(t.shape)}")
+        if isinstance(lr, torch.Tensor) and lr.numel() != 1:
+            raise RuntimeError(f"lr must be a scalar, got {tuple(lr.shape)}")
+        if scale_t is not None and scale_t.numel() != 1:
+            raise RuntimeError(f"scale_t must be a scalar, got {tuple(scale_t.shape)}")
         if not self._params:
             return
         if self._params[0].device != self._master.device:
@@ -289,7 +290,8 @@ class SodAdamW:
         if self._plan is None:
             self._step_cpu(lr, grad_scale, scale_t)
             return
-        self.update_decay()
+        if [g["weight_decay"] for g in self.groups] != self._plan_wd:
+            self.update_decay()
         lr_t = _NONE
         if isinstance(lr, torch.Tensor):
             if lr.is_cuda:

@@ -50,10 +50,11 @@ def grad_norm(grads: Sequence[torch.Tensor], prescale: float = 1.0,
                          "loss_scale")
     if growth_interval < 1:
         raise ValueError(f"growth_interval must be positive, got {growth_interval}")
-    for what, t in (("loss_scale", loss_scale), ("good_steps", good_steps),
-                    ("skips", skips)):
-        if t is not None and t.numel() != 1:
-            raise ValueError(f"{what} must be a scalar, got {tuple(t.shape)}")
+    if loss_scale is not None:
+        for t in (loss_scale, good_steps, skips):
+            if t is not None and t.numel() != 1:
+                raise ValueError(f"loss_scale, good_steps and skips must be a "
+                                 f"scalar each, got {tuple(t.shape)}")
     if grads[0].is_cuda:
         norm, mult = ext().grad_norm(
             grads, prescale, max_norm,
