@@ -313,18 +313,6 @@ SOD_DEVINL float grid(unsigned c) {
 // exception for 0 take five operations and the sign two more.
 struct Tables { float m[256], r[256]; };
 
-// sqrt(v) correctly rounded, v a float32 under 2^63: the product with 1/sqrt
-// and one step of Heron's iteration, its residual exact, in place of sqrtf's
-// look at both neighbours.  The factors of 2^64 and 2^-32 keep the residual
-// of the smallest v a normal number; checked for every v.
-SOD_DEVINL float root(float v) {
-    float u = v * 0x1p64f;
-    float y = __builtin_amdgcn_rsqf(fmaxf(u, 0x1p-90f));    // 0 gives 0
-    float q = u * y;
-    float e = __builtin_fmaf(-q, q, u);
-    return __builtin_fmaf(e, 0.5f * y, q) * 0x1p-32f;
-}
-
 // the largest bits over 32 lanes (floats >= 0 compare like their bits, and
 // NaN above all); the exchanges stay in the vector registers
 SOD_DEVINL unsigned max32lanes(unsigned v) {
@@ -408,7 +396,7 @@ SOD_DEVINL void step8(const Args &a, const Info &I, const Row &R, int tensor,
         float x = gf[e >> 2][e & 3] * gs;
         m[e] = a.fb1 * m0 + a.fc1 * x;
         v[e] = a.fb2 * (r0 * r0) + (a.fc2 * x) * x;
-        r[e] = root(v[e]);
+        r[e] = root_f32(v[e]);
         mm = fmaxf(mm, fabsf(m[e]));
         mr = max(mr, __float_as_uint(r[e]));
     }

@@ -21,6 +21,20 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// sqrt(v) correctly rounded, v a float32 from 0 up to 2^63: the product with
+// 1/sqrt and one step of Heron's iteration, its residual exact, in place of
+// sqrtf's look at both neighbours.  The factors of 2^64 and 2^-32 keep the
+// residual of the smallest v a normal number.  tools/root_f32.hip checks it for
+// every v (profiles/root_f32.log).
+SOD_DEVINL float root_f32(float v) {
+#pragma clang fp contract(off)
+    float u = v * 0x1p64f;
+    float y = __builtin_amdgcn_rsqf(fmaxf(u, 0x1p-90f));    // 0 gives 0
+    float q = u * y;
+    float e = __builtin_fmaf(-q, q, u);
+    return __builtin_fmaf(e, 0.5f * y, q) * 0x1p-32f;
+}
+
 // ---------------------------------------------------------------------------
 // Element traits: bf16 / fp16 / fp32 <-> float conversions
 // ---------------------------------------------------------------------------
