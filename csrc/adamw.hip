@@ -3,8 +3,7 @@
 //
 // The step, t counting the steps from one, every operation in float32 and
 // rounded by itself in this order (no contraction: the step gives the same
-// bits as the same operations one at a time, on any device, and so on every
-// rank):
+// bits as the same operations one at a time on the CPU, and so on every rank):
 //
 //   g = float(grad) * (grad_scale * scale)
 //   m = b1*m + (1-b1)*g              v = b2*v + ((1-b2)*g)*g
@@ -16,9 +15,9 @@
 //
 // It is bound by memory: 28 bytes an element, 16 with moments in 8 bits.  What
 // moves once a step passes the caches by (non-temporal), in whole lines:
-//   24.5M bfloat16 parameters   32 bits 107 us, 6.4 TB/s   8 bits 63 us, 6.2
-//   391M, float32 / bfloat16            1.84 ms, 6.0               1.02 ms, 6.2
-// where a large copy reaches 5.1 to 5.4 TB/s and a fill 6.9.
+//   24.5M bfloat16 parameters   32 bits 110 us, 6.3 TB/s   8 bits 62 us, 6.3
+//   391M, float32 / bfloat16            1.72 ms, 6.4               1.00 ms, 6.3
+// where a large copy reaches 5.1 to 5.5 TB/s and a fill 6.9.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -98,9 +97,9 @@ template <> struct Vec4<__half> {
     typedef short type __attribute__((ext_vector_type(4), aligned(2)));
 };
 
-// A quad of a parameter or gradient.  NT: past the caches.  FULL: all four lie in the tensor, and the
-// load is the only thing that happens (converted where it is used, so that
-// nothing waits for it between this and the next load).
+// A quad of a parameter or gradient.  NT: past the caches.  FULL: all four lie
+// in the tensor, and the load is the only thing that happens (converted where
+// it is used, so that nothing waits for it between this and the next load).
 template <typename T, bool FULL, bool NT = false>
 SOD_DEVINL typename Vec4<T>::type load4(const SOD_GLOBAL T *p, long n) {
     using V = typename Vec4<T>::type;
@@ -190,9 +189,10 @@ SOD_DEVINL float moved(float w, float m, float r, float eps, const Scalars &s) {
 // A thread has one quad, so that a CU has as many workgroups as it can and
 // their loads overlap: 116 us for 24.5M bfloat16 parameters, 120 with two or
 // four quads, 132 through the caches.  The parameter is written non-temporally
-// too (115 -> 107), and read so where it is its own master (391M float32
-// 1.89 -> 1.84 ms); gradients are not, the backward pass has just left them.  The scalars go first: with the loads in front of their
-// barrier tensors at odd addresses took 198 us and not 184, the others 1 % less.
+// too (116 -> 110), and read so where it is its own master (391M float32,
+// 3 % less); gradients are not, the backward pass has just left them.  The
+// scalars go first: with the loads in front of their barrier tensors at odd
+// addresses took 8 % more, the others 1 % less.
 
 template <typename P, typename G, bool FULL>
 SOD_DEVINL void step32(const Args &a, const Info &I, const Row &R, int tensor,
@@ -295,11 +295,12 @@ adamw32_kernel(const Args a, float *__restrict__ m, float *__restrict__ v) {
 // r is stored and not v: its codes then span 31.9 octaves of v, the next
 // step's sqrt(v) needs no second root, and it never rounds to zero unless it
 // is zero, which would leave m / eps.  A gradient that is not finite makes
-// its block's scales, and so its states, not finite.
+// its block's scales, and so its states, not finite; so does one whose square
+// is not, and the codes of such a block say nothing.
 //
 // Done plainly this is bound by its arithmetic, some 160 operations an element
 // where memory leaves time for 115: 99 us for 24.5M bfloat16 parameters.  With
-// the table, the root and the coding below it is 68, and 63 with the codes past
+// the table, the root and the coding below it is 68, and 62 with the codes past
 // the caches (and the loads in front of the scalars' barrier; behind it 1 %
 // slower).  194M float32 parameters, their own masters, take 516 us read past
 // the caches, 564 through them.  Quotients stay the compiler's, exact ones.

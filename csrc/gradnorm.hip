@@ -11,10 +11,10 @@
 // and a second kernel adds them in a fixed order (no atomics), so a repeated
 // call gives the same bits.
 //
-// Bound by memory where there is much (1.56G bfloat16: 455 us, 6.9 TB/s), by
-// the two dependent launches where there is little: 24.5M bfloat16 take 14 us,
-// 11 and 3 of them the launches', where their bytes take 9.  A next chunk
-// loaded while one is added up changes neither.
+// Bound by memory where there is much (1.56G bfloat16: 459 us, 6.8 TB/s), by
+// the two dependent launches where there is little: 24.5M bfloat16 take 14 us
+// where their bytes take 9 (12 and 4 us, each launch traced by itself).  A next
+// chunk loaded while one is added up changes neither.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
