@@ -5,8 +5,16 @@ it also passes under pytest-xdist, but the gloo spawn tests want a couple
 of cores each (worker intraop threads are pinned to 2 in test_parallel_gloo
 for exactly that reason)."""
 
+import multiprocessing.context
+
 import pytest
 import torch
+
+from value_queue import ValueQueue
+
+# the spawn tests' workers end right after they hand their tensors over
+multiprocessing.context.SpawnContext.SimpleQueue = (
+    lambda self: ValueQueue(ctx=self.get_context()))
 
 
 def pytest_configure(config):
